@@ -121,8 +121,41 @@ enum {
      *     (the order of the additions, and so the rounding, is not fixed) */
     PLOW_DOP_MOE_GLU_FP8_BLOCK128          = 188,
     PLOW_DOP_MOE_QUANT_FP8_BLOCK128        = 189,
-    PLOW_DOP_MOE_DOWN_FP8_BLOCK128         = 190
+    PLOW_DOP_MOE_DOWN_FP8_BLOCK128         = 190,
+    /* Extensions of this library, numbered far above the reference's ops (it has no counterpart of them).
+     *
+     * Products with 4-bit integer weights and group scales ("int4g"): W u8 [N][K / 2], low nibble = even k; S bf16 or
+     * f16 [N][K / G]; Z u8 [N][K / G] with zero points 0..15, or absent: 8 everywhere. w[n][k] = (q - z) * s. The
+     * group field is G (32, 64 or 128) | PLOW_W4_SCALE_F16 when the scales are f16. K is a multiple of G, N any.
+     * Products of bf16 activations with the exact integers q - z, f32 sums, scales applied in f32 per group.
+     * Activations are finite: a row of x that holds an infinity or NaN gives infinities or NaN in its own row of out
+     * (an infinity's sign is not kept: the kernels multiply q + 16 and take (z + 16) x off again). x and the W tensors are 16-byte aligned, S is 2-byte aligned.
+     * GEMM_W4:     t0=out [M][N] t1=x bf16 [M][K] t2=W t3=S t4=Z?  i0=M i1=N i2=K i3=group field i4=x pitch in
+     *              elements (0 = K, a multiple of 8) i5=out pitch in elements (0 = N) i6=0 bf16 out, 1 f32 out
+     * GEMM_GLU_W4: t0=out bf16 [M][N] t1=x t2=Wg t3=Sg t4=Zg? t5=Wu t6=Su t7=Zu?  i0=M i1=N i2=K i3=group field
+     *              i4=x pitch i5=activation (0 - 4, immediates in fj[0], fj[1]) i6=out pitch */
+    PLOW_DOP_X_GEMM_W4                     = 0x7001,
+    PLOW_DOP_X_GEMM_GLU_W4                 = 0x7002,
+    /* Log probabilities of tokens from rows of logits, with c = fj[0] (0 reads as 1; positive and finite) multiplying
+     * every logit (1 / temperature):
+     *   t1=logits [T][pitch] (bf16, or f32 with PLOW_LOGPROB_F32 in i5)
+     *   t0=f32 [T][n]: log probability of token t2[r][j] (u32 [T][n]). Token 0xFFFFFFFF asks for nothing (0 is
+     *      written), any other id >= V gives NaN
+     *   t3=f32 [T]? entropy in nats   t6=f32 [T]? log of the sum of exp(c * logit)
+     *   t4=u32 [T][A]? t5=f32 [T][A]?: the A tokens of the largest logits, best first, equal logits by lowest id, and
+     *      their log probabilities (either may be absent)
+     *   t7=u32 [T][mask pitch]?: bit i % 32 of word i / 32 set = token i is allowed
+     *   i0=T i1=V i2=n i3=A (at most PLOW_LOGPROB_MAX_ALT) i4=logits pitch in elements (0 = V) i5=flags
+     *   i6=mask pitch in words (0 = ceil(V / 32))
+     * A token that the mask forbids, or whose logit is -inf, has no probability: its log probability is -inf and it
+     * is never an alternative (lists run out into id 0xFFFFFFFF, -inf), whatever a forbidden token's logit is. A row
+     * with no token left: log of the sum -inf, entropy 0. An allowed NaN or +inf makes the row's f32 outputs NaN
+     * (both rank ahead of every number, NaN first). Logits are aligned to their element; f32 sums throughout. */
+    PLOW_DOP_X_LOGPROB                     = 0x7010
 };
+#define PLOW_W4_SCALE_F16 0x10000u    /* group field: the scales are f16, else bf16 */
+#define PLOW_LOGPROB_F32 1u           /* i5 of PLOW_DOP_X_LOGPROB: f32 logits, else bf16 */
+#define PLOW_LOGPROB_MAX_ALT 64u
 
 /* Op 180 with i7 = PLOW_ROUTER_RAW_MARK: the decode router's score with its top-k in one launch
  * (crates/packet/src/dev.rs:90-94, runtime/amd/router_decode.hip:1-63; plowrt routes such an op to
@@ -135,7 +168,16 @@ enum {
 #define PLOW_ROUTER_RAW_MARK 0x52545241u
 
 /* Weight encodings (i3 on ops 85/86, i6 on ops 48/49; dev_isa.h:442-461, :691-702). */
-enum { PLOW_MOE_ENC_BF16 = 0, PLOW_MOE_ENC_FP8BLK = 1, PLOW_MOE_ENC_MXFP4 = 2 };
+enum {
+    PLOW_MOE_ENC_BF16 = 0, PLOW_MOE_ENC_FP8BLK = 1, PLOW_MOE_ENC_MXFP4 = 2,
+    /* An extension of this library: 4-bit integers with group scales (see PLOW_DOP_X_GEMM_W4), bf16 activations.
+     * wtab / stab as on the other encodings, plus an optional zero-point table ztab u64 [E][3] (absent: 8 everywhere):
+     *   48 / 49  i6 = 16, i7 = group field, t5 = ztab?   (49 zeroes the rows of slots no expert serves)
+     *   85       i3 = 16, i7 = arm 0, i6 = group field, t6 = ztab?
+     *   86       i3 = 16, i7 = arm 0, i6 = group field, t5 = ztab?
+     * I and H are multiples of G. An expert is resident when its W and S (and Z, where ztab is bound) are non-null. */
+    PLOW_MOE_ENC_INT4G = 16
+};
 
 /* Arms of ops 85/86 (i7; runtime/amd/interp.hip:6500-6604). 0, 1 and 2/3 are the reference's; 8 is
  * this library's name for "mxfp4 weights, bf16 activations" on gathered rows (the arithmetic of the

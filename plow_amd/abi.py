@@ -41,7 +41,16 @@ OP_MOE_GLU_FP8_BLOCK128 = 188
 OP_MOE_QUANT_FP8_BLOCK128 = 189
 OP_MOE_DOWN_FP8_BLOCK128 = 190
 
+# extensions of this library: 4-bit integer weights with group scales, log probabilities of tokens
+OP_X_GEMM_W4 = 0x7001
+OP_X_GEMM_GLU_W4 = 0x7002
+OP_X_LOGPROB = 0x7010
+
 ENC_BF16, ENC_FP8BLK, ENC_MXFP4 = 0, 1, 2
+ENC_INT4G = 16                     # extension: int4 with group scales; the group field = G | W4_SCALE_F16
+W4_SCALE_F16 = 0x10000
+LOGPROB_F32 = 1
+LOGPROB_MAX_ALT = 64
 ARM_A16, ARM_W8A8, ARM_W8A8_P16, ARM_W8A8_SPLIT, ARM_W8A8_SPLIT_P16, ARM_W8A8_XQ, ARM_W4A16 = 0, 2, 3, 4, 5, 6, 8
 ARM_A4W4, ARM_A4W4_P16 = 0, 1     # enc 2: fp4 on both operands (the reference's default for mxfp4); DOWN with a bf16 part
 ROUTER_RAW_MARK = 0x52545241       # op 180 i7: the score carries its top-k (one launch)

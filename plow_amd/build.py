@@ -30,6 +30,8 @@ SOURCES = {
     "experts_a16.hip": [],
     "experts_gemv.hip": [],
     "experts_w8a8_tiled.hip": [],
+    "w4.hip": [],
+    "logprob.hip": [],
     "api.hip": [],
     "device.hip": [],
 }

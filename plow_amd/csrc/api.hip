@@ -287,12 +287,145 @@ static bool sort_reusable(const Hint& h, const void* table, uint32_t nslot, uint
     return h.sorted_table != nullptr && h.sorted_table == table && h.sorted_nslot == nslot && h.sorted_E == E && (!glu || h.sorted_kx == kx);
 }
 
+/* ---- 4-bit integer weights with group scales, log probabilities (extensions) ---------------------- */
+
+static bool aligned(const void* p, size_t a) { return (uintptr_t)p % a == 0u; }
+
+/* the group field of a descriptor into g; K is whole groups */
+static int w4_groups(PlowMoeCtx* c, const PlowDevInst* in, uint32_t field, GroupW4* g) {
+    g->G = field & 0xFFFFu, g->s_f16 = (field & PLOW_W4_SCALE_F16) ? 1u : 0u;
+    NEED(c, (field & ~(0xFFFFu | PLOW_W4_SCALE_F16)) == 0u && (g->G == 32u || g->G == 64u || g->G == 128u),
+         "op %u: group field 0x%x is not 32, 64 or 128 with an optional f16 scale bit", (unsigned)in->op, field);
+    NEED(c, g->N && g->K && g->K % g->G == 0u, "op %u: N %u and K %u must be non-zero, K a multiple of the group size %u", (unsigned)in->op, g->N, g->K, g->G);
+    NEED(c, g->act <= 4u, "op %u: activation %u is not served", (unsigned)in->op, g->act);
+    return 0;
+}
+
+static int run_w4_dense(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hipStream_t st, bool launch) {
+    const uint32_t* i = in->i;
+    const bool glu = in->op == PLOW_DOP_X_GEMM_GLU_W4;
+    GroupW4 g = {};
+    g.out = ten(in, T, 0), g.x = ten(in, T, 1);
+    g.w[0] = ten(in, T, 2), g.s[0] = ten(in, T, 3), g.z[0] = ten(in, T, 4);
+    g.M = i[0], g.N = i[1], g.K = i[2], g.E = 1u;
+    g.ldx = i[4] ? i[4] : g.K;
+    if (glu) {
+        g.w[1] = ten(in, T, 5), g.s[1] = ten(in, T, 6), g.z[1] = ten(in, T, 7);
+        g.act = i[5], g.f0 = in->fj[0].f, g.f1 = in->fj[1].f, g.ldo = i[6] ? i[6] : g.N;
+    } else {
+        NEED(c, in->t[5] == PLOW_TENSOR_NONE && in->t[6] == PLOW_TENSOR_NONE && in->t[7] == PLOW_TENSOR_NONE, "op %u: t5 - t7 are not operands of this op", (unsigned)in->op);
+        NEED(c, i[6] <= 1u, "op %u: output type %u is neither bf16 (0) nor f32 (1)", (unsigned)in->op, i[6]);
+        g.ldo = i[5] ? i[5] : g.N, g.out_f32 = i[6];
+    }
+    NEED(c, g.out && g.x && g.w[0] && g.s[0] && (!glu || (g.w[1] && g.s[1])), "op %u: output, input, weight and scale tensors must be bound", (unsigned)in->op);
+    NEED(c, !glu || !g.z[0] == !g.z[1], "op %u: the zero points of gate (t4) and up (t7) must be bound together", (unsigned)in->op);
+    NEED(c, g.M != 0u, "op %u: M = 0", (unsigned)in->op);
+    const int rc = w4_groups(c, in, i[3], &g);
+    if (rc) return rc;
+    NEED(c, g.ldx >= g.K && g.ldx % 8u == 0u, "op %u: x pitch %zu must be a multiple of 8, at least K %u", (unsigned)in->op, g.ldx, g.K);
+    NEED(c, g.ldo >= g.N, "op %u: out pitch %zu below N %u", (unsigned)in->op, g.ldo, g.N);
+    NEED(c, aligned(g.x, 16u) && aligned(g.w[0], 16u) && aligned(g.w[1], 16u) && aligned(g.s[0], 2u) && aligned(g.s[1], 2u) &&
+                aligned(g.out, g.out_f32 ? 4u : 2u),
+         "op %u: x and the weights must be 16-byte aligned, scales and output aligned to their elements", (unsigned)in->op);
+    if (!launch) return 0;
+    if (c->ws_base && c->stage) g.ws = c->stage, g.ws_bytes = c->stage_bytes;
+    return launch_w4(g, glu, st);
+}
+
+/* ops 48 / 49 at enc 16: slot-major rows; the slots are sorted by expert into the workspace */
+static int run_w4_slots(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hipStream_t st, bool launch, Hint& h) {
+    const uint32_t* i = in->i;
+    const bool glu = in->op == PLOW_DOP_MOE_GROUP_GLU_FP8_BLK;
+    const uint32_t nslot = i[0], kx = glu ? (i[4] ? i[4] : i[0]) : 1u;
+    GroupW4 g = {};
+    g.out = ten(in, T, 0), g.x = ten(in, T, 1), g.tab = ten(in, T, 2);
+    g.wtab = (const uint64_t*)ten(in, T, 3), g.stab = (const uint64_t*)ten(in, T, 4), g.ztab = (const uint64_t*)ten(in, T, 5);
+    g.N = i[1], g.K = i[2], g.E = i[3], g.act = glu ? i[5] : 0u, g.f0 = in->fj[0].f, g.f1 = in->fj[1].f;
+    g.ldx = g.K, g.ldo = g.N, g.out_f32 = glu ? 0u : 1u;
+    g.sel[0] = glu ? 0u : 2u, g.sel[1] = 1u;
+    g.nslot = nslot, g.kx = kx, g.zero_unserved = glu ? 0u : 1u, g.slots = nslot;
+    NEED(c, g.out && g.x && g.tab && g.wtab && g.stab, "op %u: t0 out, t1 in, t2 table, t3 weight table, t4 scale table must be bound", (unsigned)in->op);
+    NEED(c, nslot && g.E, "op %u: no slots or no experts", (unsigned)in->op);
+    const int wrc = w4_groups(c, in, i[7], &g);
+    if (wrc) return wrc;
+    NEED(c, aligned(g.x, 16u), "op %u: t1 must be 16-byte aligned", (unsigned)in->op);
+    NEED(c, g.E <= c->ws.max_e && nslot <= c->ws.max_slots, "op %u: %u slots / %u experts exceed the workspace (%u slots, %u experts)", (unsigned)in->op, nslot, g.E, c->ws.max_slots, c->ws.max_e);
+    if (!launch) return 0;
+    if (!sort_reusable(h, g.tab, nslot, g.E, kx, glu)) {
+        const int rc = launch_align(c->ws.meta, g.tab, c->ws.row_token, c->ws.row_partidx, c->ws.row_gate, (nslot + kx - 1u) / kx, g.E, kx,
+                                    c->ws.chunk_hist, c->ws.max_chunks, st);
+        if (rc) return rc;
+        h.sorted_table = g.tab, h.sorted_nslot = nslot, h.sorted_E = g.E, h.sorted_kx = kx;
+    }
+    g.meta = c->ws.meta, g.o_idx = c->ws.row_partidx;
+    g.a_idx = glu ? c->ws.row_token : c->ws.row_partidx;
+    if (!glu) g.gate = c->ws.row_gate;
+    return launch_w4(g, glu, st);
+}
+
+/* ops 85 / 86 at enc 16: rows gathered by expert (op 84) */
+static int run_w4_grouped(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hipStream_t st, bool launch, const Hint& h) {
+    const uint32_t* i = in->i;
+    const bool glu = in->op == PLOW_DOP_MOE_GROUP_GLU_PF;
+    if (i[7] != PLOW_MOE_ARM_A16) return fail(c, PLOW_MOE_EUNSUPPORTED, "op %u: int4 weights take arm 0, not %u", (unsigned)in->op, i[7]);
+    NEED(c, glu || i[5] == 0u, "op 86: the deterministic fused combine (i5) is served on the block-fp8 W8A8 arm only");
+    GroupW4 g = {};
+    g.out = ten(in, T, 0), g.x = ten(in, T, 1);
+    g.wtab = (const uint64_t*)ten(in, T, 2), g.stab = (const uint64_t*)ten(in, T, 3), g.meta = (const int32_t*)ten(in, T, 4);
+    g.ztab = (const uint64_t*)ten(in, T, glu ? 6 : 5);
+    g.N = i[0], g.K = i[1], g.E = i[2], g.act = glu ? i[5] : 0u, g.f0 = in->fj[0].f, g.f1 = in->fj[1].f;
+    g.ldx = g.K, g.ldo = g.N, g.out_f32 = glu ? 0u : 1u;
+    g.sel[0] = glu ? 0u : 2u, g.sel[1] = 1u;
+    g.slots = slots_of(in, h, 0u);
+    if (glu) g.a_idx = (const uint32_t*)ten(in, T, 5);
+    else g.o_idx = (const uint32_t*)ten(in, T, 6), g.gate = (const float*)ten(in, T, 7);
+    NEED(c, g.out && g.x && g.wtab && g.stab && g.meta && (glu ? g.a_idx != nullptr : (g.o_idx && g.gate)),
+         "op %u: output, input, wtab, stab, meta and the row maps must be bound", (unsigned)in->op);
+    NEED(c, g.E != 0u, "op %u: zero geometry", (unsigned)in->op);
+    const int rc = w4_groups(c, in, i[6], &g);
+    if (rc) return rc;
+    NEED(c, aligned(g.x, 16u), "op %u: t1 must be 16-byte aligned", (unsigned)in->op);
+    if (!launch) return 0;
+    return launch_w4(g, glu, st);
+}
+
+static int run_logprob(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hipStream_t st, bool launch) {
+    const uint32_t* i = in->i;
+    LogprobRun r = {};
+    r.T = i[0], r.V = i[1], r.n = i[2], r.A = i[3], r.pitch = i[4] ? i[4] : i[1], r.f32 = i[5] & PLOW_LOGPROB_F32;
+    r.logits = ten(in, T, 1);
+    if (r.n) r.logprob = (float*)ten(in, T, 0), r.ids = (const uint32_t*)ten(in, T, 2);
+    r.entropy = (float*)ten(in, T, 3), r.lse = (float*)ten(in, T, 6), r.mask = (const uint32_t*)ten(in, T, 7);
+    if (r.A) r.alt_ids = (uint32_t*)ten(in, T, 4), r.alt_logprob = (float*)ten(in, T, 5);
+    r.scale = in->fj[0].f == 0.0f ? 1.0f : in->fj[0].f;
+    const size_t words = ((size_t)r.V + 31u) / 32u;
+    r.mask_pitch = i[6] ? i[6] : words;
+    NEED(c, r.logits, "logprob: t1 logits must be bound");
+    NEED(c, r.T && r.V && r.V <= 0x7FFFFFFFu, "logprob: T %u and V %u must be non-zero, V below 2^31", r.T, r.V);
+    NEED(c, !r.n || (r.logprob && r.ids), "logprob: n = %u given tokens need t0 and t2", r.n);
+    NEED(c, r.A <= PLOW_LOGPROB_MAX_ALT, "logprob: %u alternatives, at most %u are served", r.A, PLOW_LOGPROB_MAX_ALT);
+    NEED(c, !r.A || r.alt_ids || r.alt_logprob, "logprob: %u alternatives need t4 or t5", r.A);
+    NEED(c, r.n || r.A || r.entropy || r.lse, "logprob: no output is asked for");
+    NEED(c, r.pitch >= r.V, "logprob: logits pitch %zu below V %u", r.pitch, r.V);
+    NEED(c, r.mask_pitch >= words, "logprob: mask pitch %zu below the %zu words of V %u", r.mask_pitch, words, r.V);
+    NEED(c, (i[5] & ~PLOW_LOGPROB_F32) == 0u && i[7] == 0u, "logprob: unknown flags 0x%x (i5) or 0x%x (i7)", i[5], i[7]);
+    NEED(c, r.scale > 0.0f && r.scale <= 3.4028235e38f, "logprob: scale (f0) must be positive and finite");
+    NEED(c, aligned(r.logits, r.f32 ? 4u : 2u) && aligned(r.logprob, 4u) && aligned(r.ids, 4u) && aligned(r.entropy, 4u) && aligned(r.lse, 4u) &&
+                aligned(r.alt_ids, 4u) && aligned(r.alt_logprob, 4u) && aligned(r.mask, 4u), "logprob: every tensor must be aligned to its element");
+    if (!launch) return 0;
+    if (c->ws_base && c->stage) r.ws = c->stage, r.ws_bytes = c->stage_bytes;
+    return launch_logprob(r, st);
+}
+
 #define ROUTE_FLAGS_SERVED (PLOW_ROUTE_SIGMOID | PLOW_ROUTE_NORM_TOPK | PLOW_ROUTE_BIAS | PLOW_ROUTE_F32_LOGIT | PLOW_ROUTE_SQRT_SOFTPLUS)
 static int run_op(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hipStream_t st, bool launch, Hint& h) {
     const uint32_t* i = in->i;
     if (launch && (in->op == PLOW_DOP_MOE_ROUTER_TOPK || in->op == PLOW_DOP_MOE_ROUTER_TOPK_PF || in->op == PLOW_DOP_GEMM_F32))
         h.sorted_table = nullptr; /* routing tables may change under the sort the workspace holds */
     switch (in->op) {
+    case PLOW_DOP_X_GEMM_W4:
+    case PLOW_DOP_X_GEMM_GLU_W4: return run_w4_dense(c, in, T, st, launch);
+    case PLOW_DOP_X_LOGPROB: return run_logprob(c, in, T, st, launch);
     case PLOW_DOP_GEMM_F32: {
         NEED(c, ten(in, T, 0) && ten(in, T, 1) && ten(in, T, 2), "op 180: t0 logits, t1 x, t2 W must be bound");
         NEED(c, i[0] && i[1] && i[2] && i[2] % 8u == 0u, "op 180: M, N, K must be non-zero and K a multiple of 8");
@@ -453,6 +586,7 @@ static int run_op(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hipStrea
         return launch_w8a8(c, h, slots_of(in, h, Tn * topk), g, false, st);
     }
     case PLOW_DOP_MOE_GROUP_GLU_PF: {
+        if (i[3] == PLOW_MOE_ENC_INT4G) return run_w4_grouped(c, in, T, st, launch, h);
         const uint32_t I = i[0], H = i[1], E = i[2], enc = i[3], arm = i[7];
         NEED(c, ten(in, T, 0) && ten(in, T, 1) && ten(in, T, 2) && ten(in, T, 4) && ten(in, T, 5),
              "op 85: t0 fu, t1 x, t2 wtab, t4 meta, t5 row_token must be bound");
@@ -577,6 +711,7 @@ static int run_op(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hipStrea
         return fail(c, PLOW_MOE_EUNSUPPORTED, "op 85: encoding %u arm %u is not served", enc, arm);
     }
     case PLOW_DOP_MOE_GROUP_DOWN_PF: {
+        if (i[3] == PLOW_MOE_ENC_INT4G) return run_w4_grouped(c, in, T, st, launch, h);
         const uint32_t H = i[0], I = i[1], E = i[2], enc = i[3], arm = i[7];
         NEED(c, ten(in, T, 0) && ten(in, T, 1) && ten(in, T, 2) && ten(in, T, 4) && ten(in, T, 6) && ten(in, T, 7),
              "op 86: t0 part, t1 fu, t2 wtab, t4 meta, t6 row_partidx, t7 row_gate must be bound");
@@ -704,6 +839,7 @@ static int run_op(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hipStrea
          * the grouped kernel with slot-major input / output rows */
         const bool pc = in->op == PLOW_DOP_MOE_EXPERT_GLU_GEMMA_FP8 || in->op == PLOW_DOP_MOE_EXPERT_DOWN_GEMMA_FP8;
         const bool glu = in->op == PLOW_DOP_MOE_GROUP_GLU_FP8_BLK || in->op == PLOW_DOP_MOE_EXPERT_GLU_GEMMA_FP8;
+        if (!pc && i[6] == PLOW_MOE_ENC_INT4G) return run_w4_slots(c, in, T, st, launch, h);
         uint32_t nslot, kx, N, K, E, enc, act;
         if (pc) { /* i0=k i1=N i2=K i3=E i5=B(0 = 1); act: i6 on the GLU (0 gelu_tanh, 1 silu) */
             nslot = i[0] * (i[5] ? i[5] : 1u); kx = i[0]; N = i[1]; K = i[2]; E = i[3];
@@ -921,6 +1057,7 @@ static uint32_t out_slots(const PlowDevInst* in) {
 /* the op keeps something in the context's staging while it runs */
 static bool uses_staging(const PlowDevInst* in) {
     if (in->op == PLOW_DOP_GEMM_GLU || in->op == PLOW_DOP_GEMM) return true;
+    if (in->op == PLOW_DOP_X_GEMM_W4 || in->op == PLOW_DOP_X_GEMM_GLU_W4 || in->op == PLOW_DOP_X_LOGPROB) return true;
     if (in->op == PLOW_DOP_MOE_GROUP_GLU_PF)
         return (in->i[3] == PLOW_MOE_ENC_FP8BLK && (in->i[7] == PLOW_MOE_ARM_W8A8_XQ || in->i[7] == PLOW_MOE_ARM_W8A8_SPLIT)) ||
                (in->i[3] == PLOW_MOE_ENC_MXFP4 && in->i[7] == PLOW_MOE_ARM_A4W4);
@@ -1087,6 +1224,7 @@ static int check_segment(PlowMoeCtx* c, const PlowDevInst* insts, uint32_t n) {
         NEED(c, g.t[0] == d.t[1], "segment: DOWN does not read the GLU's output");
         const bool a4w4 = g.i[3] == PLOW_MOE_ENC_MXFP4 && g.i[7] == PLOW_MOE_ARM_A4W4;
         if (quantized_mid || a4w4) NEED(c, g.t[7] == d.t[5], "segment: DOWN does not read the GLU's output scales");
+        if (g.i[3] == PLOW_MOE_ENC_INT4G) NEED(c, g.t[6] == d.t[5], "segment: ztab handles differ");
         if (a4w4) NEED(c, d.i[7] == PLOW_MOE_ARM_A4W4 || d.i[7] == PLOW_MOE_ARM_A4W4_P16, "segment: GLU arm %u and DOWN arm %u disagree", g.i[7], d.i[7]);
         NEED(c, (g.i[7] == PLOW_MOE_ARM_W8A8) == (d.i[7] == PLOW_MOE_ARM_W8A8 || d.i[7] == PLOW_MOE_ARM_W8A8_P16),
              "segment: GLU arm %u and DOWN arm %u disagree", g.i[7], d.i[7]);
@@ -1096,6 +1234,8 @@ static int check_segment(PlowMoeCtx* c, const PlowDevInst* insts, uint32_t n) {
     } else {
         NEED(c, g.i[1] == d.i[2] && g.i[2] == d.i[1] && g.i[3] == d.i[3], "segment: GLU (I,H,E) and DOWN (H,I,E) disagree");
         NEED(c, g.t[0] == d.t[1] && g.t[2] == d.t[2] && g.t[3] == d.t[3], "segment: fu / table / weight-table handles differ");
+        if (g.op == PLOW_DOP_MOE_GROUP_GLU_FP8_BLK && g.i[6] == PLOW_MOE_ENC_INT4G)
+            NEED(c, d.i[6] == g.i[6] && g.t[5] == d.t[5], "segment: weight encodings or ztab handles differ");
     }
     return 0;
 }

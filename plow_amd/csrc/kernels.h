@@ -208,6 +208,55 @@ int launch_group_down_a16(const GroupA16& g, hipStream_t st);
 /* wtab / stab rows {p, p, p} for the experts of one flat tensor: p = W + e * w_stride, S + e * s_stride */
 int launch_flat_tables(uint64_t* wtab, uint64_t* stab, const void* W, const void* S, uint32_t E, size_t w_stride,
                        size_t s_stride, hipStream_t st);
+/* Products with 4-bit integer weights and group scales (w4.hip). Dense (wtab NULL, w / s / z the tensors themselves, M
+ * rows) or routed experts: wtab / stab / ztab [E][3], rows by meta, a_idx and o_idx as in GroupA16, or, with tab set,
+ * straight from a routing table. Stream 0 is the only one (down, plain products) or the gate, stream 1 the up. */
+struct GroupW4 {
+    void* out;           /* GLU: bf16; else bf16, or f32 when out_f32 */
+    const void* x;       /* bf16 rows, pitch ldx elements */
+    const void* w[2];
+    const void* s[2];
+    const void* z[2];    /* NULL: zero point 8 */
+    const uint64_t* wtab;
+    const uint64_t* stab;
+    const uint64_t* ztab;
+    uint32_t sel[2];     /* table column of each stream */
+    const int32_t* meta; /* rowoff | cnt | tilep */
+    const uint32_t* a_idx;
+    const uint32_t* o_idx;
+    const float* gate;
+    uint32_t M, N, K, E, G, s_f16, act, out_f32;
+    size_t ldx, ldo;
+    float f0, f1;
+    uint32_t slots;      /* routed slots of the batch when the host knows them (0 = unknown) */
+    /* slot-major: the routing table [nslot]; output row = slot, input row = slot / kx. zero_unserved: rows of slots
+     * no expert serves are zeroed (DOWN) */
+    const void* tab;
+    uint32_t nslot, kx, zero_unserved;
+    /* scratch for partial sums of a K split (NULL: never split) */
+    void* ws;
+    size_t ws_bytes;
+};
+int launch_w4(const GroupW4& g, bool glu, hipStream_t st);
+
+/* Log probabilities of tokens (logprob.hip); every pointer but `logits` may be NULL. */
+struct LogprobRun {
+    const void* logits;
+    uint32_t T, V, n, A, f32;
+    size_t pitch, mask_pitch;
+    float scale;
+    float* logprob;
+    const uint32_t* ids;
+    float* entropy;
+    float* lse;
+    uint32_t* alt_ids;
+    float* alt_logprob;
+    const uint32_t* mask;
+    void* ws; /* scratch for rows split over workgroups (NULL: never split) */
+    size_t ws_bytes;
+};
+int launch_logprob(const LogprobRun& r, hipStream_t st);
+
 int launch_zero_skipped(float* part, const void* table, const uint64_t* wtab, const uint64_t* stab,
                         uint32_t wcols, uint32_t wsel, uint32_t nslot, uint32_t E, uint32_t H, hipStream_t st);
 
