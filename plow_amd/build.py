@@ -31,6 +31,8 @@ SOURCES = {
     "experts_gemv.hip": [],
     "experts_w8a8_tiled.hip": [],
     "w4.hip": [],
+    "w4_rows.hip": [],
+    "w4_tiled.hip": [],
     "logprob.hip": [],
     "api.hip": [],
     "device.hip": [],

@@ -319,7 +319,7 @@ static int run_w4_dense(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hi
     }
     NEED(c, g.out && g.x && g.w[0] && g.s[0] && (!glu || (g.w[1] && g.s[1])), "op %u: output, input, weight and scale tensors must be bound", (unsigned)in->op);
     NEED(c, !glu || !g.z[0] == !g.z[1], "op %u: the zero points of gate (t4) and up (t7) must be bound together", (unsigned)in->op);
-    NEED(c, g.M != 0u, "op %u: M = 0", (unsigned)in->op);
+    NEED(c, g.M != 0u && g.M <= 65535u * 128u, "op %u: M %u outside 1 .. 65535 * 128", (unsigned)in->op, g.M);
     const int rc = w4_groups(c, in, i[3], &g);
     if (rc) return rc;
     NEED(c, g.ldx >= g.K && g.ldx % 8u == 0u, "op %u: x pitch %zu must be a multiple of 8, at least K %u", (unsigned)in->op, g.ldx, g.K);
@@ -351,6 +351,7 @@ static int run_w4_slots(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hi
     NEED(c, aligned(g.x, 16u), "op %u: t1 must be 16-byte aligned", (unsigned)in->op);
     NEED(c, g.E <= c->ws.max_e && nslot <= c->ws.max_slots, "op %u: %u slots / %u experts exceed the workspace (%u slots, %u experts)", (unsigned)in->op, nslot, g.E, c->ws.max_slots, c->ws.max_e);
     if (!launch) return 0;
+    if (w4_vec_serves(g)) return launch_w4(g, glu, st); /* a handful of slots: the table itself lists the rows */
     if (!sort_reusable(h, g.tab, nslot, g.E, kx, glu)) {
         const int rc = launch_align(c->ws.meta, g.tab, c->ws.row_token, c->ws.row_partidx, c->ws.row_gate, (nslot + kx - 1u) / kx, g.E, kx,
                                     c->ws.chunk_hist, c->ws.max_chunks, st);

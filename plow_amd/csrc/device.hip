@@ -66,6 +66,7 @@ int plow_moe_device_setup(int device) {
     if (!rc) rc = plow_moe_w8a8_setup();
     if (!rc) rc = plow_moe_w8a8_tiled_setup();
     if (!rc) rc = plow_moe_a16_setup();
+    if (!rc) rc = plow_moe_w4_setup();
     void* ptr = nullptr;
     if (!rc && (hipGetSymbolAddress(&ptr, HIP_SYMBOL(scratch)) != hipSuccess || !ptr)) rc = PLOW_MOE_EDEVICE;
     (void)hipSetDevice(prev);

@@ -237,6 +237,8 @@ struct GroupW4 {
     void* ws;
     size_t ws_bytes;
 };
+/* the matrix-vector form serves this call (routed experts: straight from the table, no sort) */
+bool w4_vec_serves(const GroupW4& g);
 int launch_w4(const GroupW4& g, bool glu, hipStream_t st);
 
 /* Log probabilities of tokens (logprob.hip); every pointer but `logits` may be NULL. */

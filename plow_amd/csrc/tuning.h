@@ -81,5 +81,6 @@ int plow_moe_route_setup();
 int plow_moe_w8a8_setup();
 int plow_moe_w8a8_tiled_setup();
 int plow_moe_a16_setup();
+int plow_moe_w4_setup();
 
 #endif

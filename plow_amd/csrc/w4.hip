@@ -1,5 +1,5 @@
 /* w4.hip — products with 4-bit integer weights and group scales: dense (GEMM_W4, GEMM_GLU_W4) and routed experts
- * (ops 48 / 49 and 85 / 86 at enc 16).
+ * (ops 48 / 49 and 85 / 86 at enc 16). Dispatch between the kernel forms, and the matrix-vector form.
  *
  *   out[m][n] = sum over groups g of s[n][g] * sum_{k in g} x[m][k] * (q[n][k] - z[n][g])
  *
@@ -7,58 +7,8 @@
 #include "common.h"
 #include "kernels.h"
 #include "tuning.h"
-
-#define W4_WAVES 4u
-
-__device__ __forceinline__ float w4_scale(const void* s, size_t i, uint32_t f16) {
-    const uint16_t h = ((const uint16_t*)s)[i];
-    return f16 ? (float)__builtin_bit_cast(_Float16, h) : bf2f(h);
-}
-
-/* one weight row times one row of x, the wave's lanes taking 8 k each in turn; the sum in every lane */
-__device__ __forceinline__ float w4_dot(const uint8_t* w, const void* s, const uint8_t* z, size_t row, const bf16_t* x,
-                                        uint32_t K, uint32_t G, uint32_t f16, uint32_t lane) {
-    float acc = 0.0f;
-    const uint32_t* wr = (const uint32_t*)(w + row * (K / 2u));
-    for (uint32_t p = lane; p < K / 8u; p += WAVE) {
-        const size_t gi = row * (K / G) + p * 8u / G;
-        const float zf = z ? (float)z[gi] : 8.0f;
-        const uint32_t q = wr[p];
-        float t = 0.0f;
-#pragma unroll
-        for (uint32_t j = 0; j < 8u; j++) t = fmaf((float)((q >> (4u * j)) & 15u) - zf, bf2f(x[p * 8u + j]), t);
-        acc = fmaf(t, w4_scale(s, gi, f16), acc);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o, 64);
-    return acc;
-}
-
-/* a wave per output channel and, in turn, the rows of one expert (or the dense rows) */
-__global__ __launch_bounds__(W4_WAVES* WAVE) void k_w4_plain(GroupW4 g, uint32_t glu) {
-    const uint32_t lane = threadIdx.x & 63u, e = blockIdx.y;
-    const uint32_t n = blockIdx.x * W4_WAVES + (threadIdx.x >> 6);
-    if (n >= g.N) return;
-    const void *w[2], *s[2], *z[2];
-    for (uint32_t j = 0; j < 1u + glu; j++) {
-        w[j] = g.wtab ? (const void*)(uintptr_t)g.wtab[(size_t)e * 3u + g.sel[j]] : g.w[j];
-        s[j] = g.stab ? (const void*)(uintptr_t)g.stab[(size_t)e * 3u + g.sel[j]] : g.s[j];
-        z[j] = g.ztab ? (const void*)(uintptr_t)g.ztab[(size_t)e * 3u + g.sel[j]] : g.z[j];
-        if (!w[j] || !s[j] || (g.ztab && !z[j])) return; /* expert not resident */
-    }
-    const uint32_t r0 = g.meta ? (uint32_t)g.meta[e] : 0u, cnt = g.meta ? (uint32_t)g.meta[g.E + e] : g.M;
-    for (uint32_t r = r0 + blockIdx.z; r < r0 + cnt; r += gridDim.z) {
-        const uint32_t ai = g.a_idx ? g.a_idx[r] : r, oi = g.o_idx ? g.o_idx[r] : r;
-        if (ai == PLOW_EXPERT_UNUSED || oi == PLOW_EXPERT_UNUSED) continue;
-        const bf16_t* x = (const bf16_t*)g.x + (size_t)ai * g.ldx;
-        float v = w4_dot((const uint8_t*)w[0], s[0], (const uint8_t*)z[0], n, x, g.K, g.G, g.s_f16, lane);
-        if (glu) v = moe_glu(v, w4_dot((const uint8_t*)w[1], s[1], (const uint8_t*)z[1], n, x, g.K, g.G, g.s_f16, lane), g.act, g.f0, g.f1);
-        if (g.gate) v *= g.gate[r];
-        if (lane) continue;
-        if (g.out_f32) ((float*)g.out)[(size_t)oi * g.ldo + n] = v;
-        else ((bf16_t*)g.out)[(size_t)oi * g.ldo + n] = f2bf(v);
-    }
-}
+#include "w4_forms.h"
+#include "w4_tile.h"
 
 /* whether expert e can be served for stream column `sel` */
 __device__ __forceinline__ bool w4_resident(const GroupW4& g, uint32_t e, uint32_t sel) {
@@ -73,12 +23,233 @@ __global__ __launch_bounds__(256) void k_w4_zero_unserved(GroupW4 g) {
     for (uint32_t n = threadIdx.x; n < g.N; n += 256u) ((float*)g.out)[blockIdx.x * g.ldo + n] = 0.0f;
 }
 
-int launch_w4(const GroupW4& g, bool glu, hipStream_t st) {
-    if (!g.N || !g.K || !g.E) return PLOW_MOE_EINVAL;
-    if (g.zero_unserved) {
-        k_w4_zero_unserved<<<g.nslot, 256, 0, st>>>(g);
+/* ---- matrix-vector form: one row of x (the dense ops at one token, a routing slot) --------------------------
+ *
+ * A wave keeps its row of x in registers, 32 columns per lane and piece, already in the order in which the nibbles of a
+ * dword come out (w4_unpack), and walks a run of weight rows four at a time (GLU: gate and up of two channels): every
+ * lane loads 16 bytes of each row per 1 KB, the next four rows' loads are issued before these are multiplied, two bit
+ * operations and one v_dot2_f32_bf16 per two weights. A lane's 32 columns lie in one group: the dot product starts
+ * from -(16 + z) * (their sum of x), which takes the 16 + z off again, and is scaled once. The four rows' sums meet in
+ * a reduction of ten instructions: two cross-lane swaps leave one row per 16 lanes. */
+#define V_WAVES 4u
+
+template <int ITER, bool GLU, bool ASYM>
+struct VecRows { /* four weight rows' share of a lane */
+    v4i w[4][ITER];
+    uint16_t s[4][ITER];
+    uint8_t z[4][ASYM ? ITER : 1];
+};
+
+template <int ITER, bool GLU, bool ASYM>
+__global__ __launch_bounds__(V_WAVES* WAVE) void k_w4_vec(GroupW4 g, uint32_t chunks, uint32_t per_chunk) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t unit = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * V_WAVES + (threadIdx.x >> 6)));
+    const uint32_t row = unit / chunks, chunk = unit % chunks;
+    const uint32_t N = g.N, K = g.K;
+    constexpr uint32_t NC = GLU ? 2u : 4u; /* channels per four rows */
+    if (row >= (g.tab ? g.nslot : g.M)) return;
+    const uint32_t q_lo = chunk * per_chunk, q_all = (N + NC - 1u) / NC;
+    const uint32_t q_hi = q_lo + per_chunk < q_all ? q_lo + per_chunk : q_all;
+    if (q_lo >= q_hi) return;
+
+    const void *w[2] = {g.w[0], g.w[1]}, *s[2] = {g.s[0], g.s[1]}, *z[2] = {g.z[0], g.z[1]};
+    float gate = 1.0f;
+    uint32_t xrow = row;
+    if (g.tab) {
+        const PlowMoeRoute rt = ((const PlowMoeRoute*)g.tab)[row];
+        bool ok = rt.eid < g.E;
+        for (uint32_t j = 0; ok && j < (GLU ? 2u : 1u); j++) {
+            const size_t at = (size_t)rt.eid * 3u + g.sel[j];
+            w[j] = (const void*)(uintptr_t)g.wtab[at], s[j] = (const void*)(uintptr_t)g.stab[at];
+            z[j] = ASYM ? (const void*)(uintptr_t)g.ztab[at] : nullptr;
+            ok = w[j] && s[j] && (!ASYM || z[j]);
+        }
+        if (!ok) { /* no expert serves the slot: DOWN's rows are zero, GLU's stay */
+            if (!GLU)
+                for (uint32_t n = q_lo * NC + lane; n < q_hi * NC && n < N; n += WAVE) ((float*)g.out)[(size_t)row * g.ldo + n] = 0.0f;
+            return;
+        }
+        if (GLU) xrow = row / g.kx;
+        else gate = rt.gate;
     }
-    const uint32_t rows = g.meta ? 4u : (g.M < 1024u ? g.M : 1024u);
-    k_w4_plain<<<dim3((g.N + W4_WAVES - 1u) / W4_WAVES, g.E, rows), W4_WAVES * WAVE, 0, st>>>(g, glu ? 1u : 0u);
+
+    const uint32_t pieces = K / 32u, KG = K / g.G, gshift = g.G == 32u ? 0u : g.G == 64u ? 1u : 2u;
+    typedef const __attribute__((address_space(1))) uint8_t* gptr; /* global memory: a pointer out of a table is generic to the compiler */
+    auto load = [&](VecRows<ITER, GLU, ASYM>& b, uint32_t quad) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int st = GLU ? r & 1 : 0;
+            uint32_t ch = quad * NC + (uint32_t)(GLU ? r >> 1 : r);
+            ch = ch < N ? ch : N - 1u;
+            const gptr wr = (gptr)w[st] + (size_t)ch * (K / 2u), sr = (gptr)s[st] + (size_t)ch * KG * 2u, zr = (gptr)z[st] + (ASYM ? (size_t)ch * KG : 0u);
+#pragma unroll
+            for (int it = 0; it < ITER; it++) {
+                const uint32_t p = (uint32_t)it * 64u + lane;
+                const bool in = p < pieces;
+                b.w[r][it] = in ? __builtin_nontemporal_load((const __attribute__((address_space(1))) v4i*)(wr + (size_t)p * 16u)) : (v4i){0, 0, 0, 0};
+                b.s[r][it] = in ? *(const __attribute__((address_space(1))) uint16_t*)(sr + (p >> gshift) * 2u) : (uint16_t)0;
+                if (ASYM) b.z[r][it] = in ? zr[p >> gshift] : (uint8_t)0;
+            }
+        }
+    };
+    VecRows<ITER, GLU, ASYM> ring[2];
+    load(ring[0], q_lo);
+
+    v4i x[ITER][4];
+    float xs[ITER]; /* -24 (or, with zero points, -1) times the piece's sum of x */
+    const uint8_t* const xsrc = (const uint8_t*)g.x + (size_t)xrow * g.ldx * 2u;
+#pragma unroll
+    for (int it = 0; it < ITER; it++) {
+        const uint32_t p = (uint32_t)it * 64u + lane;
+        float v = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const v4i t = p < pieces ? *(const v4i*)(xsrc + (size_t)p * 64u + j * 16u) : (v4i){0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; i++) v = w4_dot2((uint32_t)t[i], 0x3F803F80u, v);
+            x[it][j] = w4_order(t);
+        }
+        xs[it] = ASYM ? -v : -24.0f * v;
+    }
+
+    auto finish = [&](const VecRows<ITER, GLU, ASYM>& b, uint32_t quad) {
+        float sum[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            float acc = 0.0f;
+#pragma unroll
+            for (int it = 0; it < ITER; it++) {
+                float t = ASYM ? (16.0f + (float)b.z[r][it]) * xs[it] : xs[it];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const v4i u = __builtin_bit_cast(v4i, w4_unpack((uint32_t)b.w[r][it][j]));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) t = w4_dot2((uint32_t)u[i], (uint32_t)x[it][j][i], t);
+                }
+                acc = fmaf(t, w4_f32(b.s[r][it], g.s_f16), acc);
+            }
+            sum[r] = acc;
+        }
+        /* lanes 0-31 hold row 0 (1), lanes 32-63 row 2 (3); then 16 lanes per row */
+        float h[2];
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[r]), __float_as_uint(sum[r + 2]), false, false);
+            h[r] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+        }
+        const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(h[0]), __float_as_uint(h[1]), false, false);
+        const float v = w4_run_sum<16>(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+        const uint32_t r = lane >> 4;
+        const float other = GLU ? __shfl_xor(v, 16, 64) : 0.0f;
+        const uint32_t ch = quad * NC + (GLU ? r >> 1 : r);
+        if ((lane & 15u) == 0u && (!GLU || !(r & 1u)) && ch < N) {
+            const float res = GLU ? moe_glu(v, other, g.act, g.f0, g.f1) : gate * v;
+            if (!GLU && g.out_f32) ((float*)g.out)[(size_t)row * g.ldo + ch] = res;
+            else ((bf16_t*)g.out)[(size_t)row * g.ldo + ch] = f2bf(res);
+        }
+    };
+    for (uint32_t quad = q_lo;;) {
+        if (quad + 1u < q_hi) load(ring[1], quad + 1u);
+        finish(ring[0], quad);
+        if (++quad >= q_hi) break;
+        if (quad + 1u < q_hi) load(ring[0], quad + 1u);
+        finish(ring[1], quad);
+        if (++quad >= q_hi) break;
+    }
+}
+
+#define W4_VEC_MAX_K 8192u
+/* Rows up to which the matrix-vector form is taken: a routing slot streams its expert's weights by itself */
+#define W4_VEC_MAX_SLOTS 64u
+
+bool w4_vec_serves(const GroupW4& g) {
+    if (g.K > W4_VEC_MAX_K || g.meta) return false;
+    return g.tab ? g.nslot <= W4_VEC_MAX_SLOTS : g.M == 1u;
+}
+
+template <int ITER, bool GLU>
+static int launch_vec(const GroupW4& g, uint32_t n_cu, hipStream_t st) {
+    const uint32_t rows = g.tab ? g.nslot : g.M, NC = GLU ? 2u : 4u;
+    const uint64_t quads = ((uint64_t)g.N + NC - 1u) / NC;
+    /* waves the chip holds at once, more of them where a row is short and a wave's registers few */
+    const uint64_t waves = (uint64_t)n_cu * (ITER == 1 ? 16u : 8u);
+    uint64_t per = (quads * rows + waves - 1u) / waves;
+    if (per == 0) per = 1;
+    if (per > quads) per = quads;
+    const uint64_t chunks = (quads + per - 1u) / per;
+    const uint32_t grid = (uint32_t)((chunks * rows + V_WAVES - 1u) / V_WAVES);
+    if (g.z[0] || g.ztab) k_w4_vec<ITER, GLU, true><<<grid, V_WAVES * WAVE, 0, st>>>(g, (uint32_t)chunks, (uint32_t)per);
+    else k_w4_vec<ITER, GLU, false><<<grid, V_WAVES * WAVE, 0, st>>>(g, (uint32_t)chunks, (uint32_t)per);
     return 0;
 }
+
+/* ---- K split: sum of the slices' partial results in slice order, through the activation for the GLU ---------- */
+__global__ __launch_bounds__(256) void k_w4_join(GroupW4 g, const float* __restrict__ part, uint32_t slices, uint32_t glu) {
+    const size_t plane = (size_t)g.M * g.N;
+    for (size_t i = (size_t)blockIdx.x * 256u + threadIdx.x; i < plane; i += (size_t)gridDim.x * 256u) {
+        float a = 0.0f, b = 0.0f;
+        for (uint32_t s = 0; s < slices; s++) {
+            a += part[(size_t)s * (1u + glu) * plane + i];
+            if (glu) b += part[((size_t)s * 2u + 1u) * plane + i];
+        }
+        if (glu) a = moe_glu(a, b, g.act, g.f0, g.f1);
+        const size_t m = i / g.N, at = m * g.ldo + (i - m * g.N);
+        if (g.out_f32) ((float*)g.out)[at] = a;
+        else ((bf16_t*)g.out)[at] = f2bf(a);
+    }
+}
+
+int launch_w4(const GroupW4& g, bool glu, hipStream_t st) {
+    if (!g.N || !g.K || !g.E || !g.G || g.K % g.G) return PLOW_MOE_EINVAL;
+    const uint32_t n_cu = plow_moe_n_cu();
+    if (!n_cu) return PLOW_MOE_EDEVICE;
+    if (w4_vec_serves(g)) {
+        const uint32_t it = (g.K / 32u + 63u) / 64u;
+        if (it <= 1u) return glu ? launch_vec<1, true>(g, n_cu, st) : launch_vec<1, false>(g, n_cu, st);
+        if (it <= 2u) return glu ? launch_vec<2, true>(g, n_cu, st) : launch_vec<2, false>(g, n_cu, st);
+        return glu ? launch_vec<4, true>(g, n_cu, st) : launch_vec<4, false>(g, n_cu, st);
+    }
+    if (g.wtab && !g.meta) return PLOW_MOE_EINVAL;
+    if (g.zero_unserved) k_w4_zero_unserved<<<g.nslot, 256, 0, st>>>(g);
+
+    /* rows of a tile: the fewest that cover the rows at hand (routed experts: the rows of a hit expert on average) */
+    const uint32_t hit = g.slots < g.E ? g.slots : g.E;
+    const uint32_t rows = !g.meta ? g.M : g.slots ? (g.slots + hit - 1u) / hit : 1u;
+    const uint32_t tm = rows <= 16u ? 16u : rows <= 32u ? 32u : rows <= 64u ? 64u : 128u;
+    const bool few = tm <= 32u;
+    const uint32_t tn = few ? w4_rows_channels(glu, tm) : w4_tiled_channels(glu, tm), ks = few ? w4_rows_kstep() : w4_tiled_kstep();
+    const uint32_t nt = (g.N + tn - 1u) / tn, steps = (g.K + ks - 1u) / ks;
+    W4Tiles tl = {};
+    uint64_t gy = 1u;
+    if (!g.meta) {
+        gy = ((uint64_t)g.M + tm - 1u) / tm;
+        /* few tiles: K split over workgroups until every CU has two, two steps each at least */
+        const uint64_t tiles = nt * gy, want = 2u * n_cu;
+        if (g.ws && tiles < n_cu && steps >= 4u) {
+            uint32_t slices = (uint32_t)((want + tiles - 1u) / tiles);
+            if (slices > steps / 2u) slices = steps / 2u;
+            const uint64_t plane = (uint64_t)g.M * g.N * (glu ? 2u : 1u) * 4u;
+            if (plane * slices > g.ws_bytes) slices = (uint32_t)(g.ws_bytes / plane);
+            if (slices >= 2u) {
+                tl.steps_per = (steps + slices - 1u) / slices;
+                tl.slices = (steps + tl.steps_per - 1u) / tl.steps_per;
+                tl.part = (float*)g.ws;
+            }
+        }
+    } else if (few) {
+        gy = g.E;
+    } else {
+        gy = (uint64_t)g.slots / tm + hit;
+        if (gy <= 65535u) tl.row_tiles = (uint32_t)gy;
+        else gy = g.E;
+    }
+    if (gy > 65535u) return PLOW_MOE_EINVAL;
+    const dim3 grid(nt, (uint32_t)gy, tl.slices ? tl.slices : 1u);
+    const int rc = few ? w4_rows_launch(g, tl, glu, tm, grid, st) : w4_tiled_launch(g, tl, glu, tm, grid, st);
+    if (rc || !tl.slices) return rc;
+    const uint64_t blocks = ((uint64_t)g.M * g.N + 255u) / 256u;
+    k_w4_join<<<(uint32_t)(blocks < 4096u ? blocks : 4096u), 256, 0, st>>>(g, tl.part, tl.slices, glu ? 1u : 0u);
+    return 0;
+}
+
+int plow_moe_w4_setup() { return w4_rows_setup() && w4_tiled_setup() ? 0 : PLOW_MOE_EDEVICE; }

@@ -1,0 +1,398 @@
+/* w4_tile.h — the matrix-unit kernel of the int4 group-scale products (w4.hip), instantiated by w4_rows.hip (a few
+ * rows) and w4_tiled.hip (many rows).
+ *
+ * A workgroup computes TM rows x TN output channels (GLU: gate and up of TN channels) over a range of K, in steps of
+ * KS columns. Rows of x are the A operand of v_mfma_f32_16x16x32_bf16 and weights the B operand, so a lane's four
+ * results are four rows of ONE channel and a group's scale is one value per lane.
+ *
+ * Weights as operands. A nibble q becomes the bf16 value 16 + q by bit operations alone (mantissa bits 3..6 of
+ * 2^4: two operations per two weights, exact), and what that adds comes off through the C operand of the group's first
+ * matrix instruction: C = -(16 + z) * sum of the row's x over the group, whose sums are made once where x is staged.
+ * Products are exact in f32; the group's sum is scaled in f32 and added to the accumulator. (Rounding q * s to bf16
+ * instead would cost 2^-9 per weight.) The pairs that come out of a dword are nibbles (i, i + 4): x is staged in the
+ * same order inside every 8 columns.
+ *
+ * Groups. A lane (channel c = lane & 15, quarter q = lane >> 4) reads 16 bytes = 32 columns of its channel per
+ * 128-column block: columns 32 q .. Instruction r multiplies dword r of all four quarters, which lie in one group only
+ * if G = 128. For G = 64 two and for G = 32 four cross-lane swaps per 16 bytes re-deal the dwords so that instruction r
+ * covers columns of one group; w4_koff says which, and the x operand is read accordingly.
+ *
+ * Staging. Weights, x, scales and zero points of the next D steps are on their way in registers (plain loads, whole
+ * 64- or 128-byte runs per row); a step is written to one of two LDS buffers, one barrier per step that orders LDS
+ * only. What lies behind K, behind the last row or the last channel is staged as zero, so that every step runs whole. */
+#ifndef PLOW_MOE_W4_TILE_H
+#define PLOW_MOE_W4_TILE_H
+
+#include "common.h"
+#include "kernels.h"
+
+/* K split of the dense products: the workgroups of slice z take the steps [z * steps_per, ...) and write f32 sums to
+ * part [slices][streams][M][N]; 0 slices = no split */
+struct W4Tiles {
+    uint32_t slices, steps_per;
+    float* part;
+    uint32_t row_tiles; /* experts: an upper bound of the row tiles over all experts (grid.y), 0 = grid.y is the expert */
+};
+
+__device__ __forceinline__ float w4_f32(uint32_t h, uint32_t f16) {
+    return f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : __uint_as_float(h << 16);
+}
+
+/* column, inside a 128-column block, of the first of the 8 values that instruction r takes from quarter q */
+template <int G>
+__device__ __forceinline__ uint32_t w4_koff(uint32_t q, uint32_t r) {
+    if (G == 128) return 32u * q + 8u * r;
+    if (G == 64) return (q < 2u ? 32u * q : 32u * (q - 2u) + 16u) + 8u * (r & 1u) + 64u * (r >> 1);
+    return 32u * r + 8u * q;
+}
+/* re-deals a lane's four dwords between the quarters so that they fit w4_koff */
+template <int G>
+__device__ __forceinline__ void w4_deal(uint32_t (&d)[4]) {
+    if (G == 128) return;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const auto s = __builtin_amdgcn_permlane32_swap(d[j], d[j + 2], false, false);
+        d[j] = s[0], d[j + 2] = s[1];
+    }
+    if (G == 64) return;
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+        const auto s = __builtin_amdgcn_permlane16_swap(d[j], d[j + 1], false, false);
+        d[j] = s[0], d[j + 1] = s[1];
+    }
+}
+/* 8 nibbles -> 8 bf16 values 16 + q, in the order (0, 4), (1, 5), (2, 6), (3, 7) */
+__device__ __forceinline__ v8bf w4_unpack(uint32_t w) {
+    v4i r;
+    r[0] = (int)(((w << 3) & 0x00780078u) | 0x41804180u);
+    r[1] = (int)(((w >> 1) & 0x00780078u) | 0x41804180u);
+    r[2] = (int)(((w >> 5) & 0x00780078u) | 0x41804180u);
+    r[3] = (int)(((w >> 9) & 0x00780078u) | 0x41804180u);
+    return __builtin_bit_cast(v8bf, r);
+}
+/* the same order for 8 staged values of x */
+__device__ __forceinline__ v4i w4_order(v4i x) {
+    v4i r;
+    r[0] = (int)__builtin_amdgcn_perm((uint32_t)x[2], (uint32_t)x[0], 0x05040100u);
+    r[1] = (int)__builtin_amdgcn_perm((uint32_t)x[2], (uint32_t)x[0], 0x07060302u);
+    r[2] = (int)__builtin_amdgcn_perm((uint32_t)x[3], (uint32_t)x[1], 0x05040100u);
+    r[3] = (int)__builtin_amdgcn_perm((uint32_t)x[3], (uint32_t)x[1], 0x07060302u);
+    return r;
+}
+__device__ __forceinline__ float w4_dot2(uint32_t a, uint32_t b, float acc) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, a), __builtin_bit_cast(v2bf, b), acc, false);
+}
+template <int CTRL>
+__device__ __forceinline__ float w4_dpp_sum(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+/* sum over aligned runs of LANES (4, 8, 16) lanes, in each of them */
+template <int LANES>
+__device__ __forceinline__ float w4_run_sum(float v) {
+    v = w4_dpp_sum<0xB1>(v); /* quad_perm 1,0,3,2 */
+    v = w4_dpp_sum<0x4E>(v); /* quad_perm 2,3,0,1 */
+    if (LANES >= 8) v = w4_dpp_sum<0x141>(v); /* row_half_mirror */
+    if (LANES >= 16) v = w4_dpp_sum<0x140>(v); /* row_mirror */
+    return v;
+}
+
+template <int WT_, int WC_, int MTW_, int NBW_, int NS_, int KS_, int D_, int G_, bool ASYM_>
+struct W4Cfg {
+    static constexpr int WT = WT_, WC = WC_, MTW = MTW_, NBW = NBW_, NS = NS_, KS = KS_, D = D_, G = G_;
+    static constexpr bool ASYM = ASYM_;
+    static constexpr int THREADS = WT * WC * 64, TM = WT * MTW * 16, TN = WC * NBW * 16;
+    static constexpr int GS = KS / G;                      /* groups per step */
+    static constexpr int XP = KS / 8, WP = KS / 32;        /* 16-byte pieces per row and step */
+    static constexpr int XL = TM * XP / THREADS, WL = NS * TN * WP / THREADS; /* pieces a thread stages */
+    static constexpr int SL = (NS * TN + THREADS - 1) / THREADS;
+    static constexpr int XROW = KS * 2 + 16, WROW = KS / 2 + 16; /* LDS row pitches: rows 4 banks apart */
+    static constexpr int X_BYTES = TM * XROW, W_BYTES = NS * TN * WROW, XS_BYTES = GS * TM * 4, S_BYTES = GS * NS * TN * 4;
+    static constexpr int BUF = X_BYTES + W_BYTES + XS_BYTES + S_BYTES * (ASYM ? 2 : 1);
+    static constexpr int LDS = 2 * BUF;
+    static_assert(TM * XP % THREADS == 0 && NS * TN * WP % THREADS == 0 && XL >= 1 && WL >= 1, "whole pieces per thread");
+    static_assert(NS * TN <= THREADS || NS * TN % THREADS == 0, "a thread stages whole channels' scales");
+    static_assert(THREADS % XP == 0 && XP % (G / 8) == 0, "a group's pieces lie in neighbouring lanes");
+};
+
+/* what a thread has on its way for one step */
+template <class C>
+struct W4Stage {
+    v4i x[C::XL], w[C::WL];
+    uint32_t s[C::SL][(C::GS + 1) / 2]; /* pairs of 16-bit scales */
+    uint32_t z[C::SL][C::ASYM ? (C::GS + 3) / 4 : 1];
+};
+
+template <class C>
+__device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uint8_t* lds, uint32_t e, uint32_t r0, uint32_t cnt,
+                                        uint32_t rb, uint32_t n0, uint32_t slice) {
+    constexpr int G = C::G, KS = C::KS, NS = C::NS;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, q = lane >> 4;
+    const uint32_t wv = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t wt = wv / C::WC, wc = wv % C::WC;
+    const uint32_t K = g.K, N = g.N, KG = K / (uint32_t)G;
+    const uint32_t steps = (K + KS - 1u) / KS;
+    const uint32_t s_lo = tl.slices ? slice * tl.steps_per : 0u;
+    const uint32_t s_hi = tl.slices ? (s_lo + tl.steps_per < steps ? s_lo + tl.steps_per : steps) : steps;
+
+    /* ---- where this thread's pieces come from ---- */
+    const uint8_t* xsrc[C::XL];
+    bool xok[C::XL];
+    const uint32_t xp = tid % C::XP;
+#pragma unroll
+    for (int j = 0; j < C::XL; j++) {
+        const uint32_t t = rb + (tid + (uint32_t)j * C::THREADS) / C::XP;
+        uint32_t ai = PLOW_EXPERT_UNUSED;
+        if (t < cnt) ai = g.a_idx ? g.a_idx[r0 + t] : r0 + t;
+        xok[j] = ai != PLOW_EXPERT_UNUSED;
+        xsrc[j] = (const uint8_t*)g.x + ((size_t)(xok[j] ? ai : 0u) * g.ldx + xp * 8u) * 2u;
+    }
+    auto tensor = [&](const uint64_t* tab, const void* const* direct, uint32_t st) -> const uint8_t* {
+        return g.wtab ? (tab ? (const uint8_t*)(uintptr_t)tab[(size_t)e * 3u + g.sel[st]] : nullptr) : (const uint8_t*)direct[st];
+    };
+    const uint8_t* wsrc[C::WL];
+    const uint32_t wp = tid % C::WP;
+#pragma unroll
+    for (int j = 0; j < C::WL; j++) {
+        const uint32_t row = (tid + (uint32_t)j * C::THREADS) / C::WP, st = NS == 2 ? row / C::TN : 0u, ch = n0 + row % C::TN;
+        wsrc[j] = tensor(g.wtab, g.w, st) + (size_t)(ch < N ? ch : N - 1u) * (K / 2u) + wp * 16u;
+    }
+    const uint16_t* ssrc[C::SL];
+    const uint8_t* zsrc[C::SL];
+    const bool szmine = NS * C::TN >= C::THREADS || tid < (uint32_t)(NS * C::TN);
+#pragma unroll
+    for (int j = 0; j < C::SL; j++) {
+        const uint32_t row = szmine ? tid + (uint32_t)j * C::THREADS : 0u, st = NS == 2 ? row / C::TN : 0u, ch = n0 + row % C::TN;
+        const size_t at = (size_t)(ch < N ? ch : N - 1u) * KG;
+        ssrc[j] = (const uint16_t*)tensor(g.stab, g.s, st) + at;
+        zsrc[j] = C::ASYM ? tensor(g.ztab, g.z, st) + at : nullptr;
+    }
+
+    auto load = [&](W4Stage<C>& b, uint32_t step) {
+        const uint32_t k0 = step * KS;
+        const bool whole = k0 + KS <= K;
+#pragma unroll
+        for (int j = 0; j < C::WL; j++)
+            b.w[j] = whole || k0 + wp * 32u < K ? *(const v4i*)(wsrc[j] + (size_t)step * (KS / 2)) : (v4i){0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < C::XL; j++)
+            b.x[j] = xok[j] && (whole || k0 + xp * 8u < K) ? *(const v4i*)(xsrc[j] + (size_t)step * (KS * 2)) : (v4i){0, 0, 0, 0};
+        if (!szmine) return;
+#pragma unroll
+        for (int j = 0; j < C::SL; j++) {
+            const uint32_t g0 = step * C::GS;
+            if (whole) {
+                __builtin_memcpy(b.s[j], ssrc[j] + g0, C::GS * 2);
+                if (C::ASYM) __builtin_memcpy(b.z[j], zsrc[j] + g0, C::GS);
+            } else {
+                uint16_t s[C::GS + 1] = {};
+                uint8_t z[C::GS + 3] = {};
+#pragma unroll
+                for (int i = 0; i < C::GS; i++)
+                    if (g0 + i < KG) {
+                        s[i] = ssrc[j][g0 + i];
+                        if (C::ASYM) z[i] = zsrc[j][g0 + i];
+                    }
+                __builtin_memcpy(b.s[j], s, C::GS * 2);
+                if (C::ASYM) __builtin_memcpy(b.z[j], z, C::GS);
+            }
+        }
+    };
+    auto stage = [&](const W4Stage<C>& b, uint8_t* buf) {
+        uint8_t* const xl = buf;
+        uint8_t* const wl = buf + C::X_BYTES;
+        float* const xs = (float*)(buf + C::X_BYTES + C::W_BYTES);
+        float* const sl = (float*)(buf + C::X_BYTES + C::W_BYTES + C::XS_BYTES);
+#pragma unroll
+        for (int j = 0; j < C::WL; j++) *(v4i*)(wl + ((tid + j * C::THREADS) / C::WP) * C::WROW + wp * 16u) = b.w[j];
+#pragma unroll
+        for (int j = 0; j < C::XL; j++) {
+            const uint32_t t = (tid + j * C::THREADS) / C::XP;
+            *(v4i*)(xl + t * C::XROW + xp * 16u) = w4_order(b.x[j]);
+            float v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v = w4_dot2((uint32_t)b.x[j][i], 0x3F803F80u, v);
+            v = w4_run_sum<G / 8>(v);
+            if (xp % (G / 8) == 0u) xs[(xp / (G / 8)) * C::TM + t] = C::ASYM ? -v : -24.0f * v;
+        }
+        if (szmine) {
+#pragma unroll
+            for (int j = 0; j < C::SL; j++) {
+#pragma unroll
+                for (int i = 0; i < C::GS; i++) {
+                    sl[i * (NS * C::TN) + tid + j * C::THREADS] = w4_f32((b.s[j][i / 2] >> (16 * (i & 1))) & 0xFFFFu, g.s_f16);
+                    if (C::ASYM) sl[(C::GS + i) * (NS * C::TN) + tid + j * C::THREADS] = 16.0f + (float)((b.z[j][i / 4] >> (8 * (i & 3))) & 0xFFu);
+                }
+            }
+        }
+    };
+
+    v4f acc[NS][C::NBW][C::MTW] = {};
+    auto multiply = [&](const uint8_t* buf) {
+        const uint8_t* const xl = buf + (wt * C::MTW * 16u + c) * C::XROW;
+        const uint8_t* const wl = buf + C::X_BYTES;
+        const float* const xs = (const float*)(buf + C::X_BYTES + C::W_BYTES) + wt * C::MTW * 16u + 4u * q;
+        const float* const sl = (const float*)(buf + C::X_BYTES + C::W_BYTES + C::XS_BYTES) + wc * C::NBW * 16u + c;
+#pragma unroll
+        for (int blk = 0; blk < KS / 128; blk++) {
+            uint32_t raw[NS][C::NBW][4];
+#pragma unroll
+            for (int st = 0; st < NS; st++)
+#pragma unroll
+                for (int nb = 0; nb < C::NBW; nb++) {
+                    const v4i w = *(const v4i*)(wl + (st * C::TN + wc * C::NBW * 16u + nb * 16u + c) * C::WROW + blk * 64u + q * 16u);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) raw[st][nb][i] = (uint32_t)w[i];
+                    w4_deal<G>(raw[st][nb]);
+                }
+            constexpr int RG = G / 32; /* instructions per group */
+#pragma unroll
+            for (int gr = 0; gr < 128 / G; gr++) {
+                const int gi = blk * (128 / G) + gr;
+                v4f cx[C::MTW];
+                v8bf a[C::MTW][RG];
+#pragma unroll
+                for (int mt = 0; mt < C::MTW; mt++) {
+                    cx[mt] = *(const v4f*)(xs + gi * C::TM + mt * 16);
+#pragma unroll
+                    for (int r = 0; r < RG; r++)
+                        a[mt][r] = *(const v8bf*)(xl + mt * 16 * C::XROW + (blk * 128u + w4_koff<G>(q, gr * RG + r)) * 2u);
+                }
+#pragma unroll
+                for (int st = 0; st < NS; st++)
+#pragma unroll
+                    for (int nb = 0; nb < C::NBW; nb++) {
+                        const float s = sl[gi * (NS * C::TN) + st * C::TN + nb * 16];
+                        const float zc = C::ASYM ? sl[(C::GS + gi) * (NS * C::TN) + st * C::TN + nb * 16] : 0.0f;
+                        v8bf b[RG];
+#pragma unroll
+                        for (int r = 0; r < RG; r++) b[r] = w4_unpack(raw[st][nb][gr * RG + r]);
+#pragma unroll
+                        for (int mt = 0; mt < C::MTW; mt++) {
+                            v4f t = cx[mt];
+                            if (C::ASYM) {
+#pragma unroll
+                                for (int i = 0; i < 4; i++) t[i] *= zc;
+                            }
+#pragma unroll
+                            for (int r = 0; r < RG; r++) t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mt][r], b[r], t, 0, 0, 0);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) acc[st][nb][mt][i] = fmaf(t[i], s, acc[st][nb][mt][i]);
+                        }
+                    }
+            }
+        }
+    };
+
+    /* ---- the walk over K: D steps on their way, two LDS buffers ---- */
+    W4Stage<C> ring[C::D];
+#pragma unroll
+    for (int d = 0; d < C::D; d++)
+        if (s_lo + d < s_hi) load(ring[d], s_lo + d);
+    for (uint32_t s0 = s_lo; s0 < s_hi; s0 += C::D) {
+#pragma unroll
+        for (int d = 0; d < C::D; d++) {
+            const uint32_t s = s0 + d;
+            if (s < s_hi) { /* the same in every lane */
+                uint8_t* const buf = lds + ((s - s_lo) & 1u) * C::BUF;
+                stage(ring[d], buf);
+                if (s + C::D < s_hi) load(ring[d], s + C::D);
+                lds_barrier(); /* the other buffer's readers have left it when this is passed, two steps before it is written */
+                multiply(buf);
+            }
+        }
+    }
+
+    /* ---- results: lane holds channel c of each 16, rows 4 q + i ---- */
+#pragma unroll
+    for (int mt = 0; mt < C::MTW; mt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t t = rb + (wt * C::MTW + mt) * 16u + 4u * q + i;
+            if (t >= cnt) continue;
+            if (tl.slices) {
+#pragma unroll
+                for (int st = 0; st < NS; st++)
+#pragma unroll
+                    for (int nb = 0; nb < C::NBW; nb++) {
+                        const uint32_t n = n0 + (wc * C::NBW + nb) * 16u + c;
+                        if (n < N) tl.part[(((size_t)slice * NS + st) * g.M + t) * N + n] = acc[st][nb][mt][i];
+                    }
+                continue;
+            }
+            const uint32_t r = r0 + t, oi = g.o_idx ? g.o_idx[r] : r;
+            if (oi == PLOW_EXPERT_UNUSED || (g.a_idx && g.a_idx[r] == PLOW_EXPERT_UNUSED)) continue;
+            const float gate = g.gate ? g.gate[r] : 1.0f;
+#pragma unroll
+            for (int nb = 0; nb < C::NBW; nb++) {
+                const uint32_t n = n0 + (wc * C::NBW + nb) * 16u + c;
+                if (n >= N) continue;
+                const float v = NS == 2 ? moe_glu(acc[0][nb][mt][i], acc[NS - 1][nb][mt][i], g.act, g.f0, g.f1) : gate * acc[0][nb][mt][i];
+                if (NS == 1 && g.out_f32) ((float*)g.out)[(size_t)oi * g.ldo + n] = v;
+                else ((bf16_t*)g.out)[(size_t)oi * g.ldo + n] = f2bf(v);
+            }
+        }
+}
+
+/* grid: x = channel tiles, y = expert (its row tiles one after the other) or, with tl.row_tiles, row tile over all
+ * experts, or dense row tile; z = K slice */
+template <class C>
+__global__ __launch_bounds__(C::THREADS) void k_w4_tile(GroupW4 g, W4Tiles tl) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t w4_lds[];
+    const uint32_t n0 = blockIdx.x * C::TN;
+    if (!g.meta) {
+        w4_tile<C>(g, tl, w4_lds, 0u, 0u, g.M, blockIdx.y * C::TM, n0, blockIdx.z);
+        return;
+    }
+    uint32_t e = blockIdx.y, rb = 0u, rows = 0xFFFFFFFFu;
+    if (tl.row_tiles) { /* which expert's which tile: the row tiles counted off in expert order */
+        uint32_t want = blockIdx.y;
+        const uint32_t lane = threadIdx.x & 63u;
+        bool found = false;
+        for (uint32_t e0 = 0; e0 < g.E; e0 += WAVE) {
+            const uint32_t n = e0 + lane < g.E ? ((uint32_t)g.meta[g.E + e0 + lane] + C::TM - 1u) / C::TM : 0u;
+            uint32_t inc = n;
+#pragma unroll
+            for (uint32_t o = 1; o < WAVE; o <<= 1) {
+                const uint32_t v = __shfl_up(inc, o, 64);
+                if (lane >= o) inc += v;
+            }
+            const unsigned long long m = __ballot(inc > want);
+            if (m) {
+                const int at = __ffsll(m) - 1;
+                e = e0 + (uint32_t)at;
+                rb = (want - (uint32_t)__shfl((int)(inc - n), at, 64)) * C::TM;
+                rows = C::TM;
+                found = true;
+                break;
+            }
+            want -= (uint32_t)__shfl((int)inc, 63, 64);
+        }
+        if (!found) return; /* (every wave of the workgroup counts the same) */
+        e = (uint32_t)__builtin_amdgcn_readfirstlane((int)e), rb = (uint32_t)__builtin_amdgcn_readfirstlane((int)rb);
+    }
+    const uint32_t cnt = (uint32_t)g.meta[g.E + e], r0 = (uint32_t)g.meta[e];
+    if (rb >= cnt) return;
+    for (int st = 0; st < C::NS; st++) {
+        const size_t at = (size_t)e * 3u + g.sel[st];
+        if (!g.wtab[at] || !g.stab[at] || (C::ASYM && !g.ztab[at])) return; /* not resident */
+    }
+    if (rows == 0xFFFFFFFFu) {
+        for (; rb < cnt; rb += C::TM) {
+            w4_tile<C>(g, tl, w4_lds, e, r0, cnt, rb, n0, 0u);
+            lds_barrier(); /* the next tile's first step may write the buffer that a slower wave still reads */
+        }
+    } else {
+        w4_tile<C>(g, tl, w4_lds, e, r0, cnt, rb, n0, 0u);
+    }
+}
+
+template <class C>
+static int w4_launch(const GroupW4& g, const W4Tiles& tl, dim3 grid, hipStream_t st) {
+    k_w4_tile<C><<<grid, C::THREADS, C::LDS, st>>>(g, tl);
+    return 0;
+}
+template <class C>
+static bool w4_setup() {
+    return hipFuncSetAttribute((const void*)k_w4_tile<C>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS) == hipSuccess;
+}
+#endif

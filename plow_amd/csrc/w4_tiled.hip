@@ -1,0 +1,31 @@
+/* w4_tiled.hip — int4 group-scale products of many rows (w4_tile.h): tiles of 64 or 128 rows x 256 channels (GLU: 128
+ * channels of gate and up), a wave per 64 rows x 64 weight rows, so that a weight unpacked feeds four matrix
+ * instructions and a row read from LDS four. */
+#include "w4_forms.h"
+#include "w4_tile.h"
+
+template <int WT, int NS, int G, bool ASYM>
+using Cfg = W4Cfg<WT, 4, 4, NS == 2 ? 2 : 4, NS, 128, 1, G, ASYM>;
+
+uint32_t w4_tiled_channels(bool glu, uint32_t) { return glu ? 128u : 256u; }
+uint32_t w4_tiled_kstep() { return 128u; }
+
+template <int WT, int NS, int G>
+static int by_zero(const GroupW4& g, const W4Tiles& tl, dim3 grid, hipStream_t st) {
+    return (g.ztab || g.z[0]) ? w4_launch<Cfg<WT, NS, G, true>>(g, tl, grid, st) : w4_launch<Cfg<WT, NS, G, false>>(g, tl, grid, st);
+}
+template <int WT, int NS>
+static int by_group(const GroupW4& g, const W4Tiles& tl, dim3 grid, hipStream_t st) {
+    return g.G == 32u ? by_zero<WT, NS, 32>(g, tl, grid, st) : g.G == 64u ? by_zero<WT, NS, 64>(g, tl, grid, st) : by_zero<WT, NS, 128>(g, tl, grid, st);
+}
+int w4_tiled_launch(const GroupW4& g, const W4Tiles& tl, bool glu, uint32_t rows, dim3 grid, hipStream_t st) {
+    if (rows == 64u) return glu ? by_group<1, 2>(g, tl, grid, st) : by_group<1, 1>(g, tl, grid, st);
+    return glu ? by_group<2, 2>(g, tl, grid, st) : by_group<2, 1>(g, tl, grid, st);
+}
+
+template <int WT, int NS>
+static bool setup2() {
+    return w4_setup<Cfg<WT, NS, 32, true>>() && w4_setup<Cfg<WT, NS, 32, false>>() && w4_setup<Cfg<WT, NS, 64, true>>() &&
+           w4_setup<Cfg<WT, NS, 64, false>>() && w4_setup<Cfg<WT, NS, 128, true>>() && w4_setup<Cfg<WT, NS, 128, false>>();
+}
+bool w4_tiled_setup() { return setup2<1, 1>() && setup2<1, 2>() && setup2<2, 1>() && setup2<2, 2>(); }
