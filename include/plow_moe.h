@@ -136,7 +136,7 @@ enum {
      *              i4=x pitch i5=activation (0 - 4, immediates in fj[0], fj[1]) i6=out pitch */
     PLOW_DOP_X_GEMM_W4                     = 0x7001,
     PLOW_DOP_X_GEMM_GLU_W4                 = 0x7002,
-    /* Log probabilities of tokens from rows of logits, with c = fj[0] (0 reads as 1; positive and finite) multiplying
+    /* Log probabilities of tokens from rows of logits, with c = fj[0] (0 reads as 1; positive, at most 1e30) multiplying
      * every logit (1 / temperature):
      *   t1=logits [T][pitch] (bf16, or f32 with PLOW_LOGPROB_F32 in i5)
      *   t0=f32 [T][n]: log probability of token t2[r][j] (u32 [T][n]). Token 0xFFFFFFFF asks for nothing (0 is
