@@ -126,7 +126,7 @@ enum {
      *
      * Products with 4-bit integer weights and group scales ("int4g"): W u8 [N][K / 2], low nibble = even k; S bf16 or
      * f16 [N][K / G]; Z u8 [N][K / G] with zero points 0..15, or absent: 8 everywhere. w[n][k] = (q - z) * s. The
-     * group field is G (32, 64 or 128) | PLOW_W4_SCALE_F16 when the scales are f16. K is a multiple of G, N any.
+     * group field is G (32, 64 or 128) | PLOW_W4_SCALE_F16 when the scales are f16. K is a multiple of G (at most 2^24), N any.
      * Products of bf16 activations with the exact integers q - z, f32 sums, scales applied in f32 per group.
      * Activations are finite: a row of x that holds an infinity or NaN gives infinities or NaN in its own row of out
      * (an infinity's sign is not kept: the kernels multiply q + 16 and take (z + 16) x off again). x and the W tensors are 16-byte aligned, S is 2-byte aligned.

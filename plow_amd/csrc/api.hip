@@ -296,7 +296,7 @@ static int w4_groups(PlowMoeCtx* c, const PlowDevInst* in, uint32_t field, Group
     g->G = field & 0xFFFFu, g->s_f16 = (field & PLOW_W4_SCALE_F16) ? 1u : 0u;
     NEED(c, (field & ~(0xFFFFu | PLOW_W4_SCALE_F16)) == 0u && (g->G == 32u || g->G == 64u || g->G == 128u),
          "op %u: group field 0x%x is not 32, 64 or 128 with an optional f16 scale bit", (unsigned)in->op, field);
-    NEED(c, g->N && g->K && g->K % g->G == 0u, "op %u: N %u and K %u must be non-zero, K a multiple of the group size %u", (unsigned)in->op, g->N, g->K, g->G);
+    NEED(c, g->N && g->K && g->K % g->G == 0u && g->K <= (1u << 24), "op %u: N %u and K %u must be non-zero, K a multiple of the group size %u, at most 2^24", (unsigned)in->op, g->N, g->K, g->G);
     NEED(c, g->act <= 4u, "op %u: activation %u is not served", (unsigned)in->op, g->act);
     return 0;
 }

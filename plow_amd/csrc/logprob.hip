@@ -24,6 +24,13 @@
 #define LP_MAX_PARTS 64u /* a lane of the joining wave each */
 typedef unsigned long long u64;
 
+/* lanes of the wave exchange data through LDS: nothing is emitted, but no read or write moves across it */
+__device__ __forceinline__ void lp_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
 /* ---- lanes exchanged within the wave, without LDS ---- */
 template <int CTRL>
 __device__ __forceinline__ uint32_t lp_dpp(uint32_t v) {
@@ -129,12 +136,13 @@ __device__ __forceinline__ void lp_scan(const LogprobRun& r, size_t row, uint32_
     uint32_t held = 0u; /* keys in the buffer */
 
     auto flush = [&]() { /* up to 64 of them into the list */
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        lp_wave_sync();
         const u64 k = lane < held ? buf[lane] : 0ull, more = lane + 64u < held ? buf[64u + lane] : 0ull;
         list = lp_merge(list, lp_sort(k));
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        lp_wave_sync();
         held = held > 64u ? held - 64u : 0u;
         if (lane < held) buf[lane] = more;
+        lp_wave_sync();
         const u64 b = lp_lane(list, A - 1u);
         bar = b > bar ? b : bar;
     };
@@ -324,10 +332,10 @@ __global__ __launch_bounds__(WAVE) void k_logprob_join(LogprobRun r, LpParts p, 
             const u64 next = mine && j < r.A && k > bar ? l[j] : 0ull;
             const bool last = __ballot(next > bar) == 0ull;
             while (held >= 64u || (last && held)) {
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                lp_wave_sync();
                 const u64 c = lane < held ? buf[lane] : 0ull, more = lane + 64u < held ? buf[64u + lane] : 0ull;
                 list = lp_merge(list, lp_sort(c));
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                lp_wave_sync();
                 held = held > 64u ? held - 64u : 0u;
                 if (lane < held) buf[lane] = more;
                 const u64 b = lp_lane(list, r.A - 1u);

@@ -112,6 +112,7 @@ __global__ __launch_bounds__(V_WAVES* WAVE) void k_w4_vec(GroupW4 g, uint32_t ch
         xs[it] = ASYM ? -v : -24.0f * v;
     }
 
+    const W4Bits bits = w4_bits();
     auto finish = [&](const VecRows<ITER, GLU, ASYM>& b, uint32_t quad) {
         float sum[4];
 #pragma unroll
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(V_WAVES* WAVE) void k_w4_vec(GroupW4 g, uint32_t ch
                 float t = ASYM ? (16.0f + (float)b.z[r][it]) * xs[it] : xs[it];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const v4i u = __builtin_bit_cast(v4i, w4_unpack((uint32_t)b.w[r][it][j]));
+                    const v4i u = __builtin_bit_cast(v4i, w4_unpack((uint32_t)b.w[r][it][j], bits));
 #pragma unroll
                     for (int i = 0; i < 4; i++) t = w4_dot2((uint32_t)u[i], (uint32_t)x[it][j][i], t);
                 }
@@ -183,6 +184,36 @@ static int launch_vec(const GroupW4& g, uint32_t n_cu, hipStream_t st) {
     return 0;
 }
 
+/* ---- tensors of fewer than 64 groups (W4_TINY_GROUPS): a thread per output ---------------------------------------- */
+__global__ __launch_bounds__(64) void k_w4_tiny(GroupW4 g, uint32_t glu) {
+    const uint32_t n = blockIdx.x * 64u + threadIdx.x, e = blockIdx.y;
+    if (n >= g.N || (g.meta && !(w4_resident(g, e, g.sel[0]) && (!glu || w4_resident(g, e, g.sel[1]))))) return;
+    const uint32_t r0 = g.meta ? (uint32_t)g.meta[e] : 0u, cnt = g.meta ? (uint32_t)g.meta[g.E + e] : g.M;
+    for (uint32_t r = r0 + blockIdx.z; r < r0 + cnt; r += gridDim.z) {
+        const uint32_t ai = g.a_idx ? g.a_idx[r] : r, oi = g.o_idx ? g.o_idx[r] : r;
+        if (ai == PLOW_EXPERT_UNUSED || oi == PLOW_EXPERT_UNUSED) continue;
+        const bf16_t* const x = (const bf16_t*)g.x + (size_t)ai * g.ldx;
+        float v[2];
+        for (uint32_t st = 0; st < 1u + glu; st++) {
+            const size_t at = (size_t)e * 3u + g.sel[st];
+            const uint8_t* const w = (g.wtab ? (const uint8_t*)(uintptr_t)g.wtab[at] : (const uint8_t*)g.w[st]) + (size_t)n * (g.K / 2u);
+            const uint16_t* const s = (g.wtab ? (const uint16_t*)(uintptr_t)g.stab[at] : (const uint16_t*)g.s[st]) + (size_t)n * (g.K / g.G);
+            const uint8_t* z = g.wtab ? (g.ztab ? (const uint8_t*)(uintptr_t)g.ztab[at] : nullptr) : (const uint8_t*)g.z[st];
+            float acc = 0.0f;
+            for (uint32_t k0 = 0, gi = 0; k0 < g.K; k0 += g.G, gi++) {
+                const float zf = z ? (float)z[(size_t)n * (g.K / g.G) + gi] : 8.0f;
+                float t = 0.0f;
+                for (uint32_t k = k0; k < k0 + g.G; k++) t = fmaf((float)((w[k / 2u] >> (4u * (k & 1u))) & 15u) - zf, bf2f(x[k]), t);
+                acc = fmaf(t, w4_f32(s[gi], g.s_f16), acc);
+            }
+            v[st] = acc;
+        }
+        const float res = glu ? moe_glu(v[0], v[1], g.act, g.f0, g.f1) : (g.gate ? g.gate[r] : 1.0f) * v[0];
+        if (g.out_f32) ((float*)g.out)[(size_t)oi * g.ldo + n] = res;
+        else ((bf16_t*)g.out)[(size_t)oi * g.ldo + n] = f2bf(res);
+    }
+}
+
 /* ---- K split: sum of the slices' partial results in slice order, through the activation for the GLU ---------- */
 __global__ __launch_bounds__(256) void k_w4_join(GroupW4 g, const float* __restrict__ part, uint32_t slices, uint32_t glu) {
     const size_t plane = (size_t)g.M * g.N;
@@ -212,12 +243,20 @@ int launch_w4(const GroupW4& g, bool glu, hipStream_t st) {
     if (g.wtab && !g.meta) return PLOW_MOE_EINVAL;
     if (g.zero_unserved) k_w4_zero_unserved<<<g.nslot, 256, 0, st>>>(g);
 
+    if ((uint64_t)g.N * (g.K / g.G) < W4_TINY_GROUPS) {
+        const uint32_t z = g.meta ? 16u : g.M < 65535u ? g.M : 65535u;
+        k_w4_tiny<<<dim3((g.N + 63u) / 64u, g.E, z), 64, 0, st>>>(g, glu ? 1u : 0u);
+        return 0;
+    }
     /* rows of a tile: the fewest that cover the rows at hand (routed experts: the rows of a hit expert on average) */
     const uint32_t hit = g.slots < g.E ? g.slots : g.E;
     const uint32_t rows = !g.meta ? g.M : g.slots ? (g.slots + hit - 1u) / hit : 1u;
     const uint32_t tm = rows <= 16u ? 16u : rows <= 32u ? 32u : rows <= 64u ? 64u : 128u;
     const bool few = tm <= 32u;
-    const uint32_t tn = few ? w4_rows_channels(glu, tm) : w4_tiled_channels(glu, tm), ks = few ? w4_rows_kstep() : w4_tiled_kstep();
+    /* 32 channels per wave while that leaves every CU two workgroups */
+    const uint64_t wide_tiles = (uint64_t)((g.N + w4_rows_channels(glu, true) - 1u) / w4_rows_channels(glu, true)) * (g.meta ? hit : (g.M + tm - 1u) / tm);
+    const bool wide = wide_tiles >= 2u * n_cu;
+    const uint32_t tn = few ? w4_rows_channels(glu, wide) : w4_tiled_channels(glu, tm), ks = few ? w4_rows_kstep() : w4_tiled_kstep();
     const uint32_t nt = (g.N + tn - 1u) / tn, steps = (g.K + ks - 1u) / ks;
     W4Tiles tl = {};
     uint64_t gy = 1u;
@@ -245,7 +284,7 @@ int launch_w4(const GroupW4& g, bool glu, hipStream_t st) {
     }
     if (gy > 65535u) return PLOW_MOE_EINVAL;
     const dim3 grid(nt, (uint32_t)gy, tl.slices ? tl.slices : 1u);
-    const int rc = few ? w4_rows_launch(g, tl, glu, tm, grid, st) : w4_tiled_launch(g, tl, glu, tm, grid, st);
+    const int rc = few ? w4_rows_launch(g, tl, glu, wide, tm, grid, st) : w4_tiled_launch(g, tl, glu, tm, grid, st);
     if (rc || !tl.slices) return rc;
     const uint64_t blocks = ((uint64_t)g.M * g.N + 255u) / 256u;
     k_w4_join<<<(uint32_t)(blocks < 4096u ? blocks : 4096u), 256, 0, st>>>(g, tl.part, tl.slices, glu ? 1u : 0u);

@@ -17,9 +17,10 @@
  * if G = 128. For G = 64 two and for G = 32 four cross-lane swaps per 16 bytes re-deal the dwords so that instruction r
  * covers columns of one group; w4_koff says which, and the x operand is read accordingly.
  *
- * Staging. Weights, x, scales and zero points of the next D steps are on their way in registers (plain loads, whole
- * 64- or 128-byte runs per row); a step is written to one of two LDS buffers, one barrier per step that orders LDS
- * only. What lies behind K, behind the last row or the last channel is staged as zero, so that every step runs whole. */
+ * Staging. Weights and x of the next D steps are on their way in registers (plain loads, whole 64- or 128-byte runs
+ * per row); a step is written to one of two LDS buffers, one barrier per step that orders LDS only. Scales and zero
+ * points come CC columns at a time, in runs of up to 64 bytes per row: read step by step, a few bytes of a line each,
+ * they cost as many requests as the weights themselves. What lies behind K, behind the last row or the last channel is staged as zero, so that every step runs whole. */
 #ifndef PLOW_MOE_W4_TILE_H
 #define PLOW_MOE_W4_TILE_H
 
@@ -61,13 +62,22 @@ __device__ __forceinline__ void w4_deal(uint32_t (&d)[4]) {
         d[j] = s[0], d[j + 1] = s[1];
     }
 }
-/* 8 nibbles -> 8 bf16 values 16 + q, in the order (0, 4), (1, 5), (2, 6), (3, 7) */
-__device__ __forceinline__ v8bf w4_unpack(uint32_t w) {
+/* 8 nibbles -> 8 bf16 values 16 + q, in the order (0, 4), (1, 5), (2, 6), (3, 7). The two constants are kept from the
+ * compiler's sight in registers: as literals they cost an instruction each, since the fused and-or takes no literal. */
+struct W4Bits {
+    uint32_t mask, base;
+};
+__device__ __forceinline__ W4Bits w4_bits() {
+    W4Bits k = {0x00780078u, 0x41804180u};
+    asm("" : "+v"(k.mask), "+s"(k.base));
+    return k;
+}
+__device__ __forceinline__ v8bf w4_unpack(uint32_t w, const W4Bits& k) {
     v4i r;
-    r[0] = (int)(((w << 3) & 0x00780078u) | 0x41804180u);
-    r[1] = (int)(((w >> 1) & 0x00780078u) | 0x41804180u);
-    r[2] = (int)(((w >> 5) & 0x00780078u) | 0x41804180u);
-    r[3] = (int)(((w >> 9) & 0x00780078u) | 0x41804180u);
+    r[0] = (int)(((w << 3) & k.mask) | k.base);
+    r[1] = (int)(((w >> 1) & k.mask) | k.base);
+    r[2] = (int)(((w >> 5) & k.mask) | k.base);
+    r[3] = (int)(((w >> 9) & k.mask) | k.base);
     return __builtin_bit_cast(v8bf, r);
 }
 /* the same order for 8 staged values of x */
@@ -96,30 +106,40 @@ __device__ __forceinline__ float w4_run_sum(float v) {
     return v;
 }
 
-template <int WT_, int WC_, int MTW_, int NBW_, int NS_, int KS_, int D_, int G_, bool ASYM_>
+/* CC: columns whose scales are staged together (a multiple of KS) */
+template <int WT_, int WC_, int MTW_, int NBW_, int NS_, int KS_, int D_, int CC_, int G_, bool ASYM_>
 struct W4Cfg {
-    static constexpr int WT = WT_, WC = WC_, MTW = MTW_, NBW = NBW_, NS = NS_, KS = KS_, D = D_, G = G_;
+    static constexpr int WT = WT_, WC = WC_, MTW = MTW_, NBW = NBW_, NS = NS_, KS = KS_, D = D_, CC = CC_, G = G_;
     static constexpr bool ASYM = ASYM_;
     static constexpr int THREADS = WT * WC * 64, TM = WT * MTW * 16, TN = WC * NBW * 16;
     static constexpr int GS = KS / G;                      /* groups per step */
     static constexpr int XP = KS / 8, WP = KS / 32;        /* 16-byte pieces per row and step */
     static constexpr int XL = TM * XP / THREADS, WL = NS * TN * WP / THREADS; /* pieces a thread stages */
-    static constexpr int SL = (NS * TN + THREADS - 1) / THREADS;
+    /* a chunk's scales and zero points of one weight row: bytes, bytes per load, loads per thread, LDS pitch (16 rows
+     * on different banks) */
+    static constexpr int CS = CC / KS, SC = CC / G, SB = SC * 2, ZB = SC, SP = SB < 16 ? SB : 16, ZP = ZB < 16 ? ZB : 16;
+    static constexpr int SN = NS * TN * (SB / SP), ZN = NS * TN * (ZB / ZP);
+    static constexpr int SL = (SN + THREADS - 1) / THREADS, ZL = (ZN + THREADS - 1) / THREADS;
+    static constexpr int SROW = SB <= 16 ? SB : SB + 16, ZROW = ZB <= 16 ? ZB : ZB + 16;
     static constexpr int XROW = KS * 2 + 16, WROW = KS / 2 + 16; /* LDS row pitches: rows 4 banks apart */
-    static constexpr int X_BYTES = TM * XROW, W_BYTES = NS * TN * WROW, XS_BYTES = GS * TM * 4, S_BYTES = GS * NS * TN * 4;
-    static constexpr int BUF = X_BYTES + W_BYTES + XS_BYTES + S_BYTES * (ASYM ? 2 : 1);
-    static constexpr int LDS = 2 * BUF;
+    static constexpr int X_BYTES = TM * XROW, W_BYTES = NS * TN * WROW, XS_BYTES = GS * TM * 4;
+    static constexpr int S_BYTES = NS * TN * SROW, Z_BYTES = ASYM ? NS * TN * ZROW : 0;
+    static constexpr int BUF = X_BYTES + W_BYTES + XS_BYTES, SBUF = S_BYTES + Z_BYTES;
+    static constexpr int LDS = 2 * BUF + 2 * SBUF; /* two buffers of a step, two of a chunk's scales */
     static_assert(TM * XP % THREADS == 0 && NS * TN * WP % THREADS == 0 && XL >= 1 && WL >= 1, "whole pieces per thread");
-    static_assert(NS * TN <= THREADS || NS * TN % THREADS == 0, "a thread stages whole channels' scales");
+    static_assert(LDS <= 160 * 1024, "two buffers fit the CU");
+    static_assert(CC % KS == 0 && CC % 128 == 0 && SP >= 4 && ZP >= 4, "a chunk is whole steps");
     static_assert(THREADS % XP == 0 && XP % (G / 8) == 0, "a group's pieces lie in neighbouring lanes");
 };
 
-/* what a thread has on its way for one step */
+/* what a thread has on its way for one step, and for one chunk's scales */
 template <class C>
 struct W4Stage {
     v4i x[C::XL], w[C::WL];
-    uint32_t s[C::SL][(C::GS + 1) / 2]; /* pairs of 16-bit scales */
-    uint32_t z[C::SL][C::ASYM ? (C::GS + 3) / 4 : 1];
+};
+template <class C>
+struct W4Scales {
+    uint32_t s[C::SL][C::SP / 4], z[C::ASYM ? C::ZL : 1][C::ZP / 4];
 };
 
 template <class C>
@@ -156,16 +176,66 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
         const uint32_t row = (tid + (uint32_t)j * C::THREADS) / C::WP, st = NS == 2 ? row / C::TN : 0u, ch = n0 + row % C::TN;
         wsrc[j] = tensor(g.wtab, g.w, st) + (size_t)(ch < N ? ch : N - 1u) * (K / 2u) + wp * 16u;
     }
-    const uint16_t* ssrc[C::SL];
-    const uint8_t* zsrc[C::SL];
-    const bool szmine = NS * C::TN >= C::THREADS || tid < (uint32_t)(NS * C::TN);
+    /* scale piece j of this thread: weight row (stream, channel) and the first of its SP bytes in the chunk */
+    auto scale_row = [&](const uint64_t* tab, const void* const* direct, uint32_t row, uint32_t elem) -> const uint8_t* {
+        const uint32_t st = NS == 2 ? row / C::TN : 0u, ch = n0 + row % C::TN;
+        return tensor(tab, direct, st) + (size_t)(ch < N ? ch : N - 1u) * KG * elem;
+    };
+    auto load_scales = [&](W4Scales<C>& b, uint32_t step) { /* of the chunk that starts with `step` */
+        const uint32_t g0 = step * C::GS;
+        const bool whole = g0 + C::SC <= KG;
 #pragma unroll
-    for (int j = 0; j < C::SL; j++) {
-        const uint32_t row = szmine ? tid + (uint32_t)j * C::THREADS : 0u, st = NS == 2 ? row / C::TN : 0u, ch = n0 + row % C::TN;
-        const size_t at = (size_t)(ch < N ? ch : N - 1u) * KG;
-        ssrc[j] = (const uint16_t*)tensor(g.stab, g.s, st) + at;
-        zsrc[j] = C::ASYM ? tensor(g.ztab, g.z, st) + at : nullptr;
-    }
+        for (int j = 0; j < C::SL; j++) {
+            const uint32_t i = tid + (uint32_t)j * C::THREADS, row = i / (C::SB / C::SP), off = (i % (C::SB / C::SP)) * C::SP;
+            if (C::SN % C::THREADS == 0 || i < (uint32_t)C::SN) {
+                const uint8_t* const p = scale_row(g.stab, g.s, row, 2u) + (size_t)g0 * 2u + off;
+                if (whole) {
+                    __builtin_memcpy(b.s[j], p, C::SP); /* rows are aligned to an element only */
+                } else {
+#pragma unroll
+                    for (uint32_t h = 0; h < C::SP / 4; h++) {
+                        const uint32_t gi = g0 + off / 2u + 2u * h;
+                        const uint32_t a = gi < KG ? *(const uint16_t*)(p + 4u * h) : 0u, c1 = gi + 1u < KG ? *(const uint16_t*)(p + 4u * h + 2u) : 0u;
+                        b.s[j][h] = a | (c1 << 16);
+                    }
+                }
+            }
+        }
+        if (!C::ASYM) return;
+#pragma unroll
+        for (int j = 0; j < C::ZL; j++) {
+            const uint32_t i = tid + (uint32_t)j * C::THREADS, row = i / (C::ZB / C::ZP), off = (i % (C::ZB / C::ZP)) * C::ZP;
+            if (C::ZN % C::THREADS == 0 || i < (uint32_t)C::ZN) {
+                const uint8_t* const p = scale_row(g.ztab, g.z, row, 1u) + g0 + off;
+                if (whole) {
+                    __builtin_memcpy(b.z[j], p, C::ZP);
+                } else {
+#pragma unroll
+                    for (uint32_t h = 0; h < C::ZP / 4; h++) {
+                        uint32_t v = 0u;
+#pragma unroll
+                        for (uint32_t i4 = 0; i4 < 4u; i4++) v |= (g0 + off + 4u * h + i4 < KG ? (uint32_t)p[4u * h + i4] : 0u) << (8u * i4);
+                        b.z[j][h] = v;
+                    }
+                }
+            }
+        }
+    };
+    auto stage_scales = [&](const W4Scales<C>& b, uint8_t* buf) {
+#pragma unroll
+        for (int j = 0; j < C::SL; j++) {
+            const uint32_t i = tid + (uint32_t)j * C::THREADS;
+            if (C::SN % C::THREADS == 0 || i < (uint32_t)C::SN)
+                __builtin_memcpy(__builtin_assume_aligned(buf + (i / (C::SB / C::SP)) * C::SROW + (i % (C::SB / C::SP)) * C::SP, C::SP), b.s[j], C::SP);
+        }
+        if (!C::ASYM) return;
+#pragma unroll
+        for (int j = 0; j < C::ZL; j++) {
+            const uint32_t i = tid + (uint32_t)j * C::THREADS;
+            if (C::ZN % C::THREADS == 0 || i < (uint32_t)C::ZN)
+                __builtin_memcpy(__builtin_assume_aligned(buf + C::S_BYTES + (i / (C::ZB / C::ZP)) * C::ZROW + (i % (C::ZB / C::ZP)) * C::ZP, C::ZP), b.z[j], C::ZP);
+        }
+    };
 
     auto load = [&](W4Stage<C>& b, uint32_t step) {
         const uint32_t k0 = step * KS;
@@ -176,32 +246,11 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
 #pragma unroll
         for (int j = 0; j < C::XL; j++)
             b.x[j] = xok[j] && (whole || k0 + xp * 8u < K) ? *(const v4i*)(xsrc[j] + (size_t)step * (KS * 2)) : (v4i){0, 0, 0, 0};
-        if (!szmine) return;
-#pragma unroll
-        for (int j = 0; j < C::SL; j++) {
-            const uint32_t g0 = step * C::GS;
-            if (whole) {
-                __builtin_memcpy(b.s[j], ssrc[j] + g0, C::GS * 2);
-                if (C::ASYM) __builtin_memcpy(b.z[j], zsrc[j] + g0, C::GS);
-            } else {
-                uint16_t s[C::GS + 1] = {};
-                uint8_t z[C::GS + 3] = {};
-#pragma unroll
-                for (int i = 0; i < C::GS; i++)
-                    if (g0 + i < KG) {
-                        s[i] = ssrc[j][g0 + i];
-                        if (C::ASYM) z[i] = zsrc[j][g0 + i];
-                    }
-                __builtin_memcpy(b.s[j], s, C::GS * 2);
-                if (C::ASYM) __builtin_memcpy(b.z[j], z, C::GS);
-            }
-        }
     };
     auto stage = [&](const W4Stage<C>& b, uint8_t* buf) {
         uint8_t* const xl = buf;
         uint8_t* const wl = buf + C::X_BYTES;
         float* const xs = (float*)(buf + C::X_BYTES + C::W_BYTES);
-        float* const sl = (float*)(buf + C::X_BYTES + C::W_BYTES + C::XS_BYTES);
 #pragma unroll
         for (int j = 0; j < C::WL; j++) *(v4i*)(wl + ((tid + j * C::THREADS) / C::WP) * C::WROW + wp * 16u) = b.w[j];
 #pragma unroll
@@ -214,24 +263,16 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
             v = w4_run_sum<G / 8>(v);
             if (xp % (G / 8) == 0u) xs[(xp / (G / 8)) * C::TM + t] = C::ASYM ? -v : -24.0f * v;
         }
-        if (szmine) {
-#pragma unroll
-            for (int j = 0; j < C::SL; j++) {
-#pragma unroll
-                for (int i = 0; i < C::GS; i++) {
-                    sl[i * (NS * C::TN) + tid + j * C::THREADS] = w4_f32((b.s[j][i / 2] >> (16 * (i & 1))) & 0xFFFFu, g.s_f16);
-                    if (C::ASYM) sl[(C::GS + i) * (NS * C::TN) + tid + j * C::THREADS] = 16.0f + (float)((b.z[j][i / 4] >> (8 * (i & 3))) & 0xFFu);
-                }
-            }
-        }
     };
 
+    const W4Bits bits = w4_bits();
     v4f acc[NS][C::NBW][C::MTW] = {};
-    auto multiply = [&](const uint8_t* buf) {
+    auto multiply = [&](const uint8_t* buf, const uint8_t* sbuf, uint32_t g0) { /* g0: the step's first group in its chunk */
         const uint8_t* const xl = buf + (wt * C::MTW * 16u + c) * C::XROW;
         const uint8_t* const wl = buf + C::X_BYTES;
         const float* const xs = (const float*)(buf + C::X_BYTES + C::W_BYTES) + wt * C::MTW * 16u + 4u * q;
-        const float* const sl = (const float*)(buf + C::X_BYTES + C::W_BYTES + C::XS_BYTES) + wc * C::NBW * 16u + c;
+        const uint8_t* const sl = sbuf + (wc * C::NBW * 16u + c) * C::SROW + g0 * 2u;
+        const uint8_t* const zl = sbuf + C::S_BYTES + (wc * C::NBW * 16u + c) * C::ZROW + g0;
 #pragma unroll
         for (int blk = 0; blk < KS / 128; blk++) {
             uint32_t raw[NS][C::NBW][4];
@@ -261,11 +302,11 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
                 for (int st = 0; st < NS; st++)
 #pragma unroll
                     for (int nb = 0; nb < C::NBW; nb++) {
-                        const float s = sl[gi * (NS * C::TN) + st * C::TN + nb * 16];
-                        const float zc = C::ASYM ? sl[(C::GS + gi) * (NS * C::TN) + st * C::TN + nb * 16] : 0.0f;
+                        const float s = w4_f32(*(const uint16_t*)(sl + (st * C::TN + nb * 16) * C::SROW + gi * 2), g.s_f16);
+                        const float zc = C::ASYM ? 16.0f + (float)zl[(st * C::TN + nb * 16) * C::ZROW + gi] : 0.0f;
                         v8bf b[RG];
 #pragma unroll
-                        for (int r = 0; r < RG; r++) b[r] = w4_unpack(raw[st][nb][gr * RG + r]);
+                        for (int r = 0; r < RG; r++) b[r] = w4_unpack(raw[st][nb][gr * RG + r], bits);
 #pragma unroll
                         for (int mt = 0; mt < C::MTW; mt++) {
                             v4f t = cx[mt];
@@ -285,6 +326,8 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
 
     /* ---- the walk over K: D steps on their way, two LDS buffers ---- */
     W4Stage<C> ring[C::D];
+    W4Scales<C> sring;
+    if (s_lo < s_hi) load_scales(sring, s_lo);
 #pragma unroll
     for (int d = 0; d < C::D; d++)
         if (s_lo + d < s_hi) load(ring[d], s_lo + d);
@@ -293,11 +336,18 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
         for (int d = 0; d < C::D; d++) {
             const uint32_t s = s0 + d;
             if (s < s_hi) { /* the same in every lane */
-                uint8_t* const buf = lds + ((s - s_lo) & 1u) * C::BUF;
+                const uint32_t n = s - s_lo, in_chunk = n % C::CS;
+                uint8_t* const buf = lds + (n & 1u) * C::BUF;
+                uint8_t* const sbuf = lds + 2 * C::BUF + ((n / C::CS) & 1u) * C::SBUF;
                 stage(ring[d], buf);
+                if (in_chunk == 0u) {
+                    stage_scales(sring, sbuf);
+                    if (s + C::CS < s_hi) load_scales(sring, s + C::CS);
+                }
                 if (s + C::D < s_hi) load(ring[d], s + C::D);
-                lds_barrier(); /* the other buffer's readers have left it when this is passed, two steps before it is written */
-                multiply(buf);
+                /* a buffer is written again two steps (chunks) later: its readers passed the barrier in between */
+                lds_barrier();
+                multiply(buf, sbuf, in_chunk * C::GS);
             }
         }
     }
