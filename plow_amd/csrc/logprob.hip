@@ -5,23 +5,27 @@
  *   logprob_i = d_i - ln Z;  entropy = ln Z - T / Z;  lse = c m + ln Z
  *
  * (the entropy comes from sums over the shifted values: no difference of large numbers). One pass over the logits: a
- * wave walks its part of a row with 4 KB of loads in flight, every lane keeps its own running maximum and both sums
- * (f32, in units of log 2; when the maximum rises by D they become 2^-D Z and 2^-D (T - D Z)), and the wave keeps the
- * best 64 tokens sorted over its lanes. A tile whose largest value lies below the A-th best token found so far, nearly
- * every one after the first few, costs the list one comparison; tokens at or above it go to a buffer of the wave, and
- * 64 of them at a time are sorted and merged into the list. The first tile's bar is the A-th largest of the 64 lanes'
- * own maxima. Tokens are ordered by a 64-bit key (value, lowest id first), so the order in which they are met does not
- * matter.
+ * wave walks its part of a row, the next 4 KB of loads under this tile's arithmetic; every lane keeps its own running
+ * maximum and both sums (f32, in units of log 2; when the maximum rises by D they become 2^-D Z and 2^-D (T - D Z)).
+ *
+ * The best A tokens: A of the row's tokens lie at or above the A-th largest of the lanes' running maxima, so what lies
+ * below that bar needs no further look: a comparison per tile. Tokens at or above it go, unsorted, to a buffer of the
+ * wave in LDS, a few dozen in all; the waves of a workgroup share the highest bar. The survivors of a row are sorted
+ * once, by 64-bit keys (value, lowest id first), so the order in which they are met does not matter. (With a sorted
+ * list per wave, 64 tokens merged at a time, one row of 120001 with 20 alternatives took 16.0 us for 12.9, 64 masked
+ * rows of 32000 with 5 took 18.4 for 14.8.)
+ * Where many tokens tie at the bar the buffer is sorted and merged into such a list after all, whose A-th key is an
+ * exact bar.
  *
  * A workgroup's four waves share a row; with few rows a row is split over up to 64 waves, whose results a second
- * launch joins (a lane per part). Sums are joined in a fixed order. */
+ * launch joins. Sums are joined in a fixed order. */
 #include "common.h"
 #include "kernels.h"
 #include "tuning.h"
 
 #define LP_WAVES 4u
 #define LP_NONE 0xFFFFFFFFu
-#define LP_MAX_PARTS 64u /* a lane of the joining wave each */
+#define LP_MAX_PARTS 64u /* a lane of a joining wave each */
 typedef unsigned long long u64;
 
 /* lanes of the wave exchange data through LDS: nothing is emitted, but no read or write moves across it */
@@ -121,119 +125,188 @@ __device__ __forceinline__ void lp_sums_wave(LpSums& s, float c2) {
     lp_sums_with<1>(s, c2), lp_sums_with<2>(s, c2), lp_sums_with<4>(s, c2), lp_sums_with<8>(s, c2), lp_sums_with<16>(s, c2), lp_sums_with<32>(s, c2);
 }
 
-/* ---- a wave's walk over vectors [lo, hi) of 16 bytes of a row; vector V / VEC is the row's ragged end ---- */
-template <bool F32, bool MASK, bool ALT>
-__device__ __forceinline__ void lp_scan(const LogprobRun& r, size_t row, uint32_t lo, uint32_t hi, float c2, u64* buf, LpSums& s, u64& list) {
-    constexpr uint32_t VEC = F32 ? 4u : 8u, U = 4u;
-    const uint32_t lane = threadIdx.x & 63u, full = r.V / VEC, tail = r.V % VEC;
-    const uint8_t* const x = (const uint8_t*)r.logits + row * r.pitch * (F32 ? 4u : 2u);
-    const uint8_t* const mk = MASK ? (const uint8_t*)(r.mask + row * r.mask_pitch) : nullptr;
-    const float NINF = -__builtin_inff();
-    const uint32_t A = ALT ? r.A : 0u;
-    s.m = NINF, s.z = 0.0f, s.t = 0.0f;
-    list = 0ull;
-    u64 bar = 0ull; /* the A-th best of the list: what is not above it cannot be among the A best */
-    uint32_t held = 0u; /* keys in the buffer */
+#define LP_BUF 256u  /* keys a wave's buffer holds */
+#define LP_KEEP 80u  /* LDS bytes of a lane's tile, 64 of them used: lanes on different banks */
+#define LP_LIST 64u  /* keys a part of a split row hands on, at least PLOW_LOGPROB_MAX_ALT */
 
-    auto flush = [&]() { /* up to 64 of them into the list */
+__device__ __forceinline__ uint32_t lp_ord(float x) { return route_ord(x); }
+__device__ __forceinline__ float lp_unord(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? o & 0x7FFFFFFFu : ~o); }
+/* a lower bound of the A-th largest of the wave's 64 values (its upper 16 bits are that value's; -inf: no bound). The
+ * values are ordered as unsigned numbers, whose bits are found from the top */
+__device__ __forceinline__ float lp_ath(float v, uint32_t A) {
+    const uint32_t k = lp_ord(v);
+    uint32_t t = 0u;
+#pragma unroll
+    for (int b = 31; b >= 16; b--) {
+        const uint32_t c = t | (1u << b);
+        t = (uint32_t)__popcll(__ballot(k >= c)) >= A ? c : t;
+    }
+    return t <= 0x007FFFFFu ? -__builtin_inff() : lp_unord(t);
+}
+
+/* The best A tokens met so far, in one wave: a buffer of tokens none of which need be among them, and, once that has
+ * run over, a list sorted over the lanes whose A-th key is `bar`. bar_v: no token with a smaller value counts. */
+struct LpBest {
+    u64 list, bar;
+    float bar_v;
+    uint32_t held, A;
+    u64* buf;
+    __device__ __forceinline__ void init(uint32_t a, u64* b) { list = 0ull, bar = 0ull, bar_v = -__builtin_inff(), held = 0u, A = a, buf = b; }
+    __device__ __forceinline__ void raise(float v) { bar_v = v > bar_v ? v : bar_v; }
+    /* the lanes' keys that `take` names (the buffer has room for 64) */
+    __device__ __forceinline__ void push(u64 k, bool take) {
+        const u64 m = __ballot(take);
+        if (take) buf[held + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u))] = k;
+        held += (uint32_t)__popcll(m);
+    }
+    __device__ __forceinline__ void prune() { /* what the bar has left behind since leaves the buffer */
+        const uint32_t lane = threadIdx.x & 63u, n = held;
+        u64 k[LP_BUF / 64u];
         lp_wave_sync();
-        const u64 k = lane < held ? buf[lane] : 0ull, more = lane + 64u < held ? buf[64u + lane] : 0ull;
-        list = lp_merge(list, lp_sort(k));
+#pragma unroll
+        for (uint32_t r = 0; r < LP_BUF / 64u; r++) k[r] = r * 64u + lane < n ? buf[r * 64u + lane] : 0ull;
         lp_wave_sync();
-        held = held > 64u ? held - 64u : 0u;
-        if (lane < held) buf[lane] = more;
+        held = 0u;
+#pragma unroll
+        for (uint32_t r = 0; r < LP_BUF / 64u; r++) push(k[r], k[r] > bar && !(lp_value(k[r]) < bar_v));
         lp_wave_sync();
-        const u64 b = lp_lane(list, A - 1u);
-        bar = b > bar ? b : bar;
+    }
+    __device__ __forceinline__ void sort_in() { /* the whole buffer into the list */
+        const uint32_t lane = threadIdx.x & 63u;
+        lp_wave_sync();
+        for (uint32_t at = 0; at < held; at += 64u) {
+            const u64 k = lp_sort(at + lane < held ? buf[at + lane] : 0ull);
+            list = lp_lane(list, 0u) == 0ull ? k : lp_merge(list, k); /* (the first 64 are the list) */
+        }
+        lp_wave_sync();
+        held = 0u;
+        bar = lp_lane(list, A - 1u);
+        if (bar) raise(lp_value(bar));
+    }
+};
+
+/* One tile of N values per lane into the sums and the best tokens. id0, id_at(i): the tile's lowest id and the id of
+ * this lane's value i; stash() keeps the lane's values where
+ * value_at(i), i not a constant, finds them; wg_bar: the workgroup's bar, as lp_ord. */
+template <int N, bool ALT, class IdAt, class Stash, class ValueAt>
+__device__ __forceinline__ void lp_tile(const float (&val)[N], LpSums& s, LpBest& best, uint32_t* wg_bar, float c2, uint32_t id0, IdAt id_at, Stash stash, ValueAt value_at) {
+    const float NINF = -__builtin_inff();
+    float top = val[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) top = fmaxf(top, val[i]); /* (passes over NaN: Z carries it) */
+    lp_rebase(s, fmaxf(s.m, top), c2);
+    const float base = s.m == NINF ? 0.0f : s.m;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float d = (val[i] - base) * c2, e = __builtin_amdgcn_exp2f(d);
+        s.z += e;
+        s.t = fmaf(e, fmaxf(d, -1000.0f), s.t); /* e = 0 there */
+    }
+    if (!ALT) return;
+
+    best.raise(lp_unord(*(volatile uint32_t*)wg_bar));
+    if (!__ballot(!(top < best.bar_v) || s.z != s.z)) return;
+    const float own = lp_ath(s.m, best.A);
+    if (own > best.bar_v) {
+        best.raise(own);
+        if ((threadIdx.x & 63u) == 0u) atomicMax(wg_bar, lp_ord(own));
+    }
+    /* above the bar, or at it unless all that still come at it have higher ids than an exact bar's; NaN is always in */
+    const bool past = best.bar_v == NINF || (best.bar != 0ull && lp_value(best.bar) == best.bar_v && ~(uint32_t)best.bar < id0);
+    const float bar = best.bar_v;
+    uint32_t mine = 0u;
+#pragma unroll
+    for (int i = 0; i < N; i++) mine |= (past ? !(val[i] <= bar) : !(val[i] < bar)) ? 1u << i : 0u;
+    /* One of each lane's at a time: most lanes have none, few have two. A register cannot be named by a number, so the
+     * lanes that have any put theirs into LDS first (read again from memory, which is busy, each turn waits for it). */
+    if (mine) stash();
+    while (__ballot(mine != 0u)) {
+        const uint32_t i = mine ? (uint32_t)__ffs((int)mine) - 1u : 0u;
+        const u64 k = mine ? lp_key(value_at(i), id_at(i)) : 0ull;
+        mine &= mine - 1u;
+        if (best.held > LP_BUF - 64u) {
+            best.prune();
+            if (best.held > LP_BUF - 64u) best.sort_in(); /* ties at the bar, a row that rises */
+        }
+        best.push(k, k > best.bar);
+    }
+}
+
+/* ---- a wave's walk over the vectors [lo, hi) of 16 bytes of a row, and with `tail` the values behind its last one ---- */
+template <bool F32, bool MASK, bool ALT>
+__device__ __forceinline__ void lp_scan(const LogprobRun& r, size_t row, uint32_t lo, uint32_t hi, bool tail, float c2, uint32_t* wg_bar, uint8_t* keep, LpSums& s, LpBest& best) {
+    constexpr uint32_t VEC = F32 ? 4u : 8u, U = 4u, N = U * VEC;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint8_t* const x = (const uint8_t*)r.logits + row * r.pitch * (F32 ? 4u : 2u);
+    const uint32_t* const mw = MASK ? r.mask + row * r.mask_pitch : nullptr;
+    const uint8_t* const mk = (const uint8_t*)mw;
+    const float NINF = -__builtin_inff();
+    s.m = NINF, s.z = 0.0f, s.t = 0.0f;
+    auto value = [&](uint32_t id) { /* one logit, as the mask leaves it */
+        if (MASK && !((mw[id >> 5] >> (id & 31u)) & 1u)) return NINF;
+        return F32 ? *(const float*)(x + (size_t)id * 4u) : bf2f(*(const bf16_t*)(x + (size_t)id * 2u));
     };
 
-    bool first = true;
-    for (uint32_t v0 = lo; v0 < hi; v0 += 64u * U) {
-        uint32_t raw[U][4], bits[U];
+    /* The next tile's loads go out ahead of this one's arithmetic, none of them under a condition: a vector past the
+     * end is the last one again and counts as -inf. */
+    uint32_t raw[2][U][4];
+    uint8_t bits[2][U];
+    auto load = [&](uint32_t b, uint32_t v0) {
 #pragma unroll
         for (uint32_t u = 0; u < U; u++) {
-            const uint32_t v = v0 + u * 64u + lane;
-            bits[u] = v < hi ? (F32 ? 0xFu : 0xFFu) : 0u; /* values of the vector that exist and are allowed */
-            if (v < hi && v < full) {
-                __builtin_memcpy(raw[u], x + (size_t)v * 16u, 16); /* rows are aligned to an element only */
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < 4u; i++) raw[u][i] = 0u;
-                if (v < hi) {
-                    bits[u] = (1u << tail) - 1u;
-                    for (uint32_t i = 0; i < tail; i++) {
-                        if (F32) {
-                            const uint32_t w = *(const uint32_t*)(x + ((size_t)v * VEC + i) * 4u);
-#pragma unroll
-                            for (uint32_t j = 0; j < 4u; j++)
-                                if (j == i) raw[u][j] = w;
-                        } else {
-                            const uint32_t w = (uint32_t)*(const uint16_t*)(x + ((size_t)v * VEC + i) * 2u) << (16u * (i & 1u));
-#pragma unroll
-                            for (uint32_t j = 0; j < 4u; j++)
-                                if (j == i / 2u) raw[u][j] |= w;
-                        }
-                    }
-                }
-            }
-            if (MASK && v < hi) bits[u] &= F32 ? (uint32_t)mk[v >> 1] >> (4u * (v & 1u)) : (uint32_t)mk[v];
+            uint32_t v = v0 + u * 64u + lane;
+            v = v < hi ? v : hi - 1u;
+            __builtin_memcpy(raw[b][u], x + (size_t)v * 16u, 16); /* rows are aligned to an element only */
+            if (MASK) bits[b][u] = F32 ? mk[v >> 1] : mk[v];
         }
-        float val[U * VEC];
-        const bool some_out = MASK || v0 + 64u * U > (hi < full ? hi : full); /* the same in every lane */
+    };
+    auto tile = [&](uint32_t b, uint32_t v0) {
+        float val[N];
 #pragma unroll
         for (uint32_t u = 0; u < U; u++)
 #pragma unroll
             for (uint32_t j = 0; j < VEC; j++)
-                val[u * VEC + j] = __uint_as_float(F32 ? raw[u][j & 3u] : (j & 1u) ? raw[u][j / 2u] & 0xFFFF0000u : raw[u][j / 2u] << 16);
-        if (some_out) {
+                val[u * VEC + j] = __uint_as_float(F32 ? raw[b][u][j & 3u] : (j & 1u) ? raw[b][u][j / 2u] & 0xFFFF0000u : raw[b][u][j / 2u] << 16);
+        if (MASK || v0 + 64u * U > hi) { /* the same in every lane */
 #pragma unroll
-            for (uint32_t u = 0; u < U; u++)
+            for (uint32_t u = 0; u < U; u++) {
+                const uint32_t v = v0 + u * 64u + lane;
+                const uint32_t ok = v >= hi ? 0u : !MASK ? 0xFFu : F32 ? (uint32_t)bits[b][u] >> (4u * (v & 1u)) : (uint32_t)bits[b][u];
 #pragma unroll
                 for (uint32_t j = 0; j < VEC; j++)
-                    if (!((bits[u] >> j) & 1u)) val[u * VEC + j] = NINF;
-        }
-        float top = val[0];
-#pragma unroll
-        for (uint32_t i = 1; i < U * VEC; i++) top = fmaxf(top, val[i]); /* (passes over NaN: Z carries it) */
-
-        lp_rebase(s, fmaxf(s.m, top), c2);
-        const float base = s.m == NINF ? 0.0f : s.m;
-#pragma unroll
-        for (uint32_t i = 0; i < U * VEC; i++) {
-            const float d = (val[i] - base) * c2, e = __builtin_amdgcn_exp2f(d);
-            s.z += e;
-            s.t = fmaf(e, fmaxf(d, -1000.0f), s.t); /* e = 0 there */
-        }
-
-        if (ALT) {
-            if (first) {
-                /* A of this tile's tokens lie at or above the A-th largest of the lanes' own best */
-                u64 best = 0ull;
-#pragma unroll
-                for (uint32_t i = 0; i < U * VEC; i++) {
-                    const u64 k = lp_key(val[i], (v0 + (i / VEC) * 64u + lane) * VEC + i % VEC);
-                    best = k > best ? k : best;
-                }
-                const u64 b = lp_lane(lp_sort(best), A - 1u);
-                bar = b ? b - 1ull : 0ull;
-                first = false;
+                    if (!((ok >> j) & 1u)) val[u * VEC + j] = NINF;
             }
-            const bool near = bar == 0ull || !(top < lp_value(bar)) || s.z != s.z;
-            if (__ballot(near && top != NINF) || __ballot(s.z != s.z)) {
+        }
+        auto id_at = [&](uint32_t i) { return (v0 + (i / VEC) * 64u + lane) * VEC + i % VEC; };
+        uint8_t* const kept = ALT ? keep + lane * LP_KEEP : nullptr; /* this lane's 64 bytes */
+        lp_tile<(int)N, ALT>(val, s, best, wg_bar, c2, v0 * VEC, id_at,
+                             [&]() {
 #pragma unroll
-                for (uint32_t i = 0; i < U * VEC; i++) {
-                    const u64 k = lp_key(val[i], (v0 + (i / VEC) * 64u + lane) * VEC + i % VEC);
-                    const u64 m = __ballot(k > bar);
-                    if (m) {
-                        if (k > bar) buf[held + (uint32_t)__popcll(m & ((1ull << lane) - 1ull))] = k;
-                        held += (uint32_t)__popcll(m);
-                        if (held >= 64u) flush();
-                    }
-                }
-            }
+                                 for (uint32_t u = 0; u < U; u++) __builtin_memcpy(__builtin_assume_aligned(kept + u * 16u, 16), raw[b][u], 16);
+                             },
+                             [&](uint32_t i) { return F32 ? *(const float*)(kept + i * 4u) : bf2f(*(const bf16_t*)(kept + i * 2u)); });
+    };
+    if (lo < hi) {
+        load(0u, lo);
+        for (uint32_t v0 = lo;;) {
+            load(1u, v0 + 64u * U);
+            tile(0u, v0);
+            if ((v0 += 64u * U) >= hi) break;
+            load(0u, v0 + 64u * U);
+            tile(1u, v0);
+            if ((v0 += 64u * U) >= hi) break;
         }
     }
-    if (ALT && held) flush();
+    if (tail) {
+        const uint32_t id0 = r.V / VEC * VEC, id = id0 + lane;
+        float val[1] = {id < r.V ? value(id) : NINF};
+        lp_tile<1, ALT>(val, s, best, wg_bar, c2, id0, [&](uint32_t) { return id; }, []() {}, [&](uint32_t) { return val[0]; });
+    }
+    if (ALT) {
+        best.raise(lp_unord(*(volatile uint32_t*)wg_bar));
+        best.prune();
+        if (lp_lane(best.list, 0u) != 0ull) best.sort_in();
+    }
     lp_sums_wave(s, c2);
 }
 
@@ -267,85 +340,132 @@ __device__ __forceinline__ void lp_write(const LogprobRun& r, size_t row, const 
     }
 }
 
-struct LpParts { /* rows split over parts: their sums and lists in scratch */
-    uint32_t n;    /* parts per row, 0 = a workgroup per row */
-    LpSums* sums;  /* [T][n] */
-    u64* lists;    /* [T][n][A] */
+/* rows split over parts: what each hands on, in scratch */
+struct LpPart {
+    LpSums sums;
+    uint32_t n; /* keys of its list */
+    float bar;  /* A tokens of the row lie at or above it */
+};
+struct LpParts {
+    uint32_t n;     /* parts per row, 0 = a workgroup per row */
+    LpPart* part;   /* [T][n] */
+    u64* lists;     /* [T][n][LP_LIST] */
 };
 
 template <bool F32, bool MASK, bool ALT>
 __global__ __launch_bounds__(LP_WAVES* WAVE) void k_logprob(LogprobRun r, LpParts p, float c2) {
-    __shared__ u64 buf[LP_WAVES][ALT ? 128 : 1];
-    __shared__ LpSums part[LP_WAVES];
+    __shared__ u64 buf[LP_WAVES][ALT ? LP_BUF : 1u];
+    __shared__ u64 last[ALT ? LP_BUF : 1u];
+    __shared__ __attribute__((aligned(16))) uint8_t keep[LP_WAVES][ALT ? WAVE * LP_KEEP : 1u];
+    __shared__ LpPart part[LP_WAVES];
+    __shared__ uint32_t wg_bar;
     const uint32_t lane = threadIdx.x & 63u, wv = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     constexpr uint32_t VEC = F32 ? 4u : 8u;
-    const uint64_t nv = (r.V + VEC - 1u) / VEC;
+    const uint64_t nv = r.V / VEC;
     const uint32_t per_row = p.n ? p.n / LP_WAVES : 1u, parts = per_row * LP_WAVES;
     const size_t row = blockIdx.x / per_row;
     const uint32_t at = (uint32_t)(blockIdx.x % per_row) * LP_WAVES + wv;
     LpSums s;
-    u64 list;
-    lp_scan<F32, MASK, ALT>(r, row, (uint32_t)(nv * at / parts), (uint32_t)(nv * (at + 1u) / parts), c2, buf[wv], s, list);
+    LpBest best;
+    if (ALT) {
+        if (threadIdx.x == 0u) wg_bar = lp_ord(-__builtin_inff());
+        __syncthreads();
+        best.init(r.A, buf[wv]);
+    }
+    lp_scan<F32, MASK, ALT>(r, row, (uint32_t)(nv * at / parts), (uint32_t)(nv * (at + 1u) / parts), r.V % VEC != 0u && at == parts - 1u, c2, &wg_bar, ALT ? &keep[wv][0] : nullptr, s, best);
+    if (ALT && best.held > (p.n ? LP_LIST : LP_BUF - 64u)) best.sort_in();
+    const bool sorted = ALT && lp_lane(best.list, 0u) != 0ull; /* then the buffer is empty */
+    const uint32_t n = !ALT ? 0u : sorted ? (uint32_t)__popcll(__ballot(best.list != 0ull)) : best.held;
     if (p.n) {
-        if (lane == 0u) p.sums[row * p.n + at] = s;
-        if (ALT && lane < r.A) p.lists[(row * p.n + at) * r.A + lane] = list;
+        if (lane == 0u) p.part[row * p.n + at] = {s, n, ALT ? best.bar_v : 0.0f};
+        if (ALT && lane < n) p.lists[(row * p.n + at) * LP_LIST + lane] = sorted ? best.list : buf[wv][lane];
         return;
     }
-    if (lane == 0u) part[wv] = s;
-    if (ALT) buf[wv][lane] = list;
+    if (ALT && sorted) buf[wv][lane] = best.list;
+    if (lane == 0u) part[wv] = {s, n, 0.0f};
     __syncthreads();
     if (wv) return;
-#pragma unroll
-    for (uint32_t w = 1; w < LP_WAVES; w++) {
-        LpSums o = part[w];
-        const float m = fmaxf(s.m, o.m);
-        lp_rebase(s, m, c2), lp_rebase(o, m, c2);
-        s.z += o.z, s.t += o.t;
-        if (ALT) list = lp_merge(list, buf[w][lane]);
+    LpBest all;
+    if (ALT) {
+        all.init(r.A, last);
+        all.raise(lp_unord(wg_bar));
     }
-    lp_write<ALT>(r, row, s, list);
+#pragma unroll 1
+    for (uint32_t w = 0; w < LP_WAVES; w++) {
+        if (w) {
+            LpSums o = part[w].sums;
+            const float m = fmaxf(s.m, o.m);
+            lp_rebase(s, m, c2), lp_rebase(o, m, c2);
+            s.z += o.z, s.t += o.t;
+        }
+        if (ALT)
+            for (uint32_t j = 0; j < part[w].n; j += 64u) {
+                const u64 k = j + lane < part[w].n ? buf[w][j + lane] : 0ull;
+                if (all.held > LP_BUF - 64u) all.sort_in();
+                all.push(k, k > all.bar && !(lp_value(k) < all.bar_v));
+            }
+    }
+    if (ALT) all.sort_in();
+    lp_write<ALT>(r, row, s, ALT ? all.list : 0ull);
 }
 
-/* a wave per row: a lane per part */
+/* a workgroup per row: 8 waves fetch the parts' lists, all of them on their way at once, and keep what lies at or above
+ * the A-th largest of the parts' maxima and above every part's own bar; one wave sorts that */
+#define LP_JOIN_WAVES 8u
 template <bool ALT>
-__global__ __launch_bounds__(WAVE) void k_logprob_join(LogprobRun r, LpParts p, float c2) {
-    __shared__ u64 buf[128];
-    const uint32_t lane = threadIdx.x;
+__global__ __launch_bounds__(ALT ? LP_JOIN_WAVES * WAVE : WAVE) void k_logprob_join(LogprobRun r, LpParts p, float c2) {
+    __shared__ u64 kept[ALT ? LP_MAX_PARTS * LP_LIST : 1u];
+    __shared__ u64 buf[ALT ? LP_BUF : 1u];
+    __shared__ uint32_t n_kept;
+    const uint32_t lane = threadIdx.x & 63u, wv = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const size_t row = blockIdx.x;
-    const bool mine = lane < p.n;
-    LpSums s = {-__builtin_inff(), 0.0f, 0.0f};
-    if (mine) s = p.sums[row * p.n + lane];
-    u64 list = 0ull;
+    u64 k[LP_MAX_PARTS / LP_JOIN_WAVES];
     if (ALT) {
-        const u64* const l = p.lists + (row * p.n + (mine ? lane : 0u)) * r.A;
-        /* A tokens lie at or above the A-th largest of the parts' own best */
-        u64 k = mine ? l[0] : 0ull;
-        u64 bar = lp_lane(lp_sort(k), r.A - 1u);
-        bar = bar ? bar - 1ull : 0ull;
-        uint32_t held = 0u;
-        for (uint32_t j = 0;;) {
-            const u64 m = __ballot(k > bar);
-            if (!m) break; /* the lists fall: nothing further on is above the bar either */
-            if (k > bar) buf[held + (uint32_t)__popcll(m & ((1ull << lane) - 1ull))] = k;
-            held += (uint32_t)__popcll(m);
-            j++;
-            const u64 next = mine && j < r.A && k > bar ? l[j] : 0ull;
-            const bool last = __ballot(next > bar) == 0ull;
-            while (held >= 64u || (last && held)) {
-                lp_wave_sync();
-                const u64 c = lane < held ? buf[lane] : 0ull, more = lane + 64u < held ? buf[64u + lane] : 0ull;
-                list = lp_merge(list, lp_sort(c));
-                lp_wave_sync();
-                held = held > 64u ? held - 64u : 0u;
-                if (lane < held) buf[lane] = more;
-                const u64 b = lp_lane(list, r.A - 1u);
-                bar = b > bar ? b : bar;
-            }
-            k = next;
+        if (threadIdx.x == 0u) n_kept = 0u;
+#pragma unroll
+        for (uint32_t j = 0; j < LP_MAX_PARTS / LP_JOIN_WAVES; j++) { /* (what lies behind a list's end is not used) */
+            const uint32_t q = j * LP_JOIN_WAVES + wv;
+            k[j] = p.lists[(row * p.n + (q < p.n ? q : 0u)) * LP_LIST + lane];
         }
     }
+    LpPart mine = {{-__builtin_inff(), 0.0f, 0.0f}, 0u, -__builtin_inff()};
+    if (lane < p.n) mine = p.part[row * p.n + lane];
+    LpSums s = mine.sums;
+    float bar = -__builtin_inff();
+    if (ALT) {
+        bar = mine.bar;
+        bar = fmaxf(bar, lp_xorf<1>(bar)), bar = fmaxf(bar, lp_xorf<2>(bar)), bar = fmaxf(bar, lp_xorf<4>(bar));
+        bar = fmaxf(bar, lp_xorf<8>(bar)), bar = fmaxf(bar, lp_xorf<16>(bar)), bar = fmaxf(bar, lp_xorf<32>(bar));
+        bar = fmaxf(bar, lp_ath(s.m, r.A));
+        __syncthreads();
+#pragma unroll
+        for (uint32_t j = 0; j < LP_MAX_PARTS / LP_JOIN_WAVES; j++) {
+            const uint32_t q = j * LP_JOIN_WAVES + wv;
+            if (q >= p.n) continue; /* the same in every lane */
+            const bool take = lane < (uint32_t)__builtin_amdgcn_readlane((int)mine.n, (int)q) && !(lp_value(k[j]) < bar);
+            const u64 m = __ballot(take);
+            if (!m) continue;
+            uint32_t at = 0u;
+            if (lane == 0u) at = atomicAdd(&n_kept, (uint32_t)__popcll(m));
+            at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+            if (take) kept[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u))] = k[j];
+        }
+        __syncthreads();
+    }
+    if (wv) return;
+    LpBest all;
+    if (ALT) {
+        all.init(r.A, buf);
+        const uint32_t n = n_kept;
+        for (uint32_t j = 0; j < n; j += 64u) {
+            const u64 c = j + lane < n ? kept[j + lane] : 0ull;
+            if (all.held > LP_BUF - 64u) all.sort_in();
+            all.push(c, c > all.bar);
+        }
+        all.sort_in();
+    }
     lp_sums_wave(s, c2);
-    lp_write<ALT>(r, row, s, list);
+    lp_write<ALT>(r, row, s, ALT ? all.list : 0ull);
 }
 
 template <bool F32, bool MASK>
@@ -366,8 +486,8 @@ int launch_logprob(const LogprobRun& r, hipStream_t st) {
     const float c2 = r.scale * 1.44269504088896341f; /* log2(e) */
     if (wgs >= 2u && r.ws) {
         const uint32_t n = wgs * LP_WAVES;
-        const size_t lists = (size_t)r.T * n * r.A * 8u, sums = (size_t)r.T * n * sizeof(LpSums);
-        if (lists + sums <= r.ws_bytes) p.n = n, p.lists = (u64*)r.ws, p.sums = (LpSums*)((uint8_t*)r.ws + lists);
+        const size_t lists = r.A ? (size_t)r.T * n * LP_LIST * 8u : 0u, parts = (size_t)r.T * n * sizeof(LpPart);
+        if (lists + parts <= r.ws_bytes) p.n = n, p.lists = (u64*)r.ws, p.part = (LpPart*)((uint8_t*)r.ws + lists);
     }
     const uint64_t grid = (uint64_t)r.T * (p.n ? p.n / LP_WAVES : 1u);
     if (grid > 0x7FFFFFFFull) return PLOW_MOE_EINVAL;
@@ -379,7 +499,7 @@ int launch_logprob(const LogprobRun& r, hipStream_t st) {
         else lp_launch<false, false>(r, p, (uint32_t)grid, c2, st);
     }
     if (p.n) {
-        if (r.A) k_logprob_join<true><<<r.T, WAVE, 0, st>>>(r, p, c2);
+        if (r.A) k_logprob_join<true><<<r.T, LP_JOIN_WAVES * WAVE, 0, st>>>(r, p, c2);
         else k_logprob_join<false><<<r.T, WAVE, 0, st>>>(r, p, c2);
     }
     return 0;

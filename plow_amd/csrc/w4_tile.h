@@ -386,7 +386,7 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
 /* grid: x = channel tiles, y = expert (its row tiles one after the other) or, with tl.row_tiles, row tile over all
  * experts, or dense row tile; z = K slice */
 template <class C>
-__global__ __launch_bounds__(C::THREADS) void k_w4_tile(GroupW4 g, W4Tiles tl) {
+__global__ __launch_bounds__(C::THREADS, 2) void k_w4_tile(GroupW4 g, W4Tiles tl) {
     extern __shared__ __attribute__((aligned(16))) uint8_t w4_lds[];
     const uint32_t n0 = blockIdx.x * C::TN;
     if (!g.meta) {
