@@ -39,6 +39,8 @@ def expert_bytes(cfg):
         return 3 * I * H + 3 * ((I + 127) // 128) * ((H + 127) // 128) * 4
     if cfg.enc == "mxfp4":
         return 3 * I * H // 2 + 3 * I * H // 32
+    if cfg.enc == "int4g":
+        return 3 * I * H // 2 + 3 * I * H // cfg.group * (3 if cfg.zero_points else 2)
     if cfg.enc == "fp8pc":
         return 3 * I * H + (2 * I + H) * 4
     return 6 * I * H
@@ -173,7 +175,7 @@ def run_cell(a, name, tokens, steps, warmup, share=None, cpu_mode="full"):
                      "frac": round(achieved_tf / mfma_peak, 4), "flops_per_launch": dom_flops}}
     rec = {
         "value": round(ms * 1e3, 2), "unit": "us/layer", "ms_per_step": round(ms, 4), "steps": steps, "warmup": warmup,
-        "dtype": {"fp8blk": "fp8_e4m3", "mxfp4": "fp4_e2m1", "fp8pc": "fp8_e4m3", "bf16": "bf16"}[cfg.enc],
+        "dtype": {"fp8blk": "fp8_e4m3", "mxfp4": "fp4_e2m1", "fp8pc": "fp8_e4m3", "bf16": "bf16", "int4g": "int4"}[cfg.enc],
         "config": {"workload": f"{cfg.name}: H={cfg.H} E={cfg.E}+{cfg.n_shared} I={cfg.I} top{cfg.k} "
                                f"T={cfg.T} enc={cfg.enc} arm={cfg.arm} groups={cfg.n_group}/{cfg.topk_group}",
                    "tokens": T, "experts_hit": hit, "rows": rows,
@@ -216,7 +218,7 @@ def cpu_baseline(a, name, cfg, dev, mode):
         if sp.role in ("scratch", "out", "table"):
             chost.alloc(nm)
     full_host = synth.to_host(dev)
-    for nm in ("Wr", "bias", "residual", "Ws_gate", "Ws_up", "Ws_down", "wtab", "stab", "ewt", "est"):
+    for nm in ("Wr", "bias", "residual", "Ws_gate", "Ws_up", "Ws_down", "wtab", "stab", "ztab", "ewt", "est"):
         if nm in full_host.t:
             chost.t[nm] = full_host.t[nm]
     if "residual" in chost.t:
@@ -251,7 +253,7 @@ def main():
     ap.add_argument("--gpus", type=int, default=1)
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--warmup", type=int, default=3)
-    ap.add_argument("--config", default="", help="one configuration only (c1..c6); default: c2 with c3 under prefill_4k")
+    ap.add_argument("--config", default="", help="one configuration only (c1..c7); default: c2 with c3 under prefill_4k")
     ap.add_argument("--tokens", type=int, default=0)
     ap.add_argument("--arm", default="", help="override the configuration's arm (a16 | w8a8 | w8a8q | w8a8atomic | w8a8det | a4w4)")
     ap.add_argument("--zipf", type=float, default=-1.0, help="override the expert popularity exponent")

@@ -532,7 +532,9 @@ static void cache_fit(RowCache* c, uint32_t rows) {
 /* 85: t0=fu_g|fq t1=xn2|xq t2=wtab t3=stab t4=meta t5=row_token t6=xs t7=fs  i0=I i1=H i2=E i3=enc
  * i4=xs pitch i5=act i7=arm. Work item = (expert, 128-channel group); slices split E*(I/128)
  * (I rounded up). */
+static void op_w4_grouped(const PlowDevInst* in, uint32_t slice, uint32_t nblk, void* const* T, int is_glu);
 static void op_group_glu(const PlowDevInst* in, uint32_t slice, uint32_t nblk, void* const* T) {
+    if (in->i[3] == PLOW_MOE_ENC_INT4G) { op_w4_grouped(in, slice, nblk, T, 1); return; }
     const uint64_t* wtab = TEN(in, T, 2);
     const uint64_t* stab = TEN(in, T, 3);
     const int32_t* meta = TEN(in, T, 4);
@@ -711,6 +713,7 @@ static void det_add(double* p, double q) {
 }
 
 static void op_group_down(const PlowDevInst* in, uint32_t slice, uint32_t nblk, void* const* T) {
+    if (in->i[3] == PLOW_MOE_ENC_INT4G) { op_w4_grouped(in, slice, nblk, T, 0); return; }
     const uint64_t* wtab = TEN(in, T, 2);
     const uint64_t* stab = TEN(in, T, 3);
     const int32_t* meta = TEN(in, T, 4);
@@ -787,7 +790,9 @@ static void op_group_down(const PlowDevInst* in, uint32_t slice, uint32_t nblk, 
 /* 48: t0=fu[B*k][I] t1=x t2=table t3=wtab t4=stab  i0=slots i1=I i2=H i3=n_exp i4=slots per x row
  * (0 = one shared row) i5=act i6=enc. Slot s reads x row s / i4. Sentinel or null base: nothing
  * written. Slices split slots*I. */
+static void op_w4_slots(const PlowDevInst* in, uint32_t slice, uint32_t nblk, void* const* T, int is_glu);
 static void op_dec_glu(const PlowDevInst* in, uint32_t slice, uint32_t nblk, void* const* T) {
+    if (in->i[6] == PLOW_MOE_ENC_INT4G) { op_w4_slots(in, slice, nblk, T, 1); return; }
     orc_bf16* fu = TEN(in, T, 0);
     const orc_bf16* x = TEN(in, T, 1);
     const PlowMoeRoute* tab = TEN(in, T, 2);
@@ -818,6 +823,7 @@ static void op_dec_glu(const PlowDevInst* in, uint32_t slice, uint32_t nblk, voi
 /* 49: t0=part[B*k][H] t1=fu t2=table t3=wtab t4=stab  i0=slots i1=H i2=I i3=n_exp i6=enc.
  * part[s] = gate_s * (Wd_e . fu[s]); sentinel or null base writes zeros. */
 static void op_dec_down(const PlowDevInst* in, uint32_t slice, uint32_t nblk, void* const* T) {
+    if (in->i[6] == PLOW_MOE_ENC_INT4G) { op_w4_slots(in, slice, nblk, T, 0); return; }
     float* part = TEN(in, T, 0);
     const orc_bf16* fu = TEN(in, T, 1);
     const PlowMoeRoute* tab = TEN(in, T, 2);
@@ -1405,6 +1411,173 @@ static void op_moe_down_block128(const PlowDevInst* in, uint32_t slice, uint32_t
     cache_free(&rc);
 }
 
+/* ---- 4-bit integer weights with group scales, log probabilities (extensions of the library; the reference has no
+ * counterpart): the definitions in binary64, one rounding at the end ------------------------------------------- */
+
+typedef struct {
+    uint32_t K, G, f16;
+} W4Fmt;
+static W4Fmt w4_fmt(uint32_t K, uint32_t field) {
+    W4Fmt f = {K, field & 0xFFFFu, (field & PLOW_W4_SCALE_F16) ? 1u : 0u};
+    return f;
+}
+static double f16_value(uint16_t h) {
+    const int e = (h >> 10) & 31, m = h & 1023;
+    const double v = e == 31 ? (m ? NAN : INFINITY) : e ? ldexp(1024.0 + m, e - 25) : ldexp((double)m, -24);
+    return (h & 0x8000u) ? -v : v;
+}
+/* <row n of W, a> with the group scales and zero points (Z may be null: 8) */
+static double w4_dot(const W4Fmt* f, const uint8_t* W, const uint16_t* S, const uint8_t* Z, uint32_t n, const orc_bf16* a) {
+    const uint32_t groups = f->K / f->G;
+    double acc = 0.0;
+    for (uint32_t g = 0; g < groups; g++) {
+        const size_t at = (size_t)n * groups + g;
+        const double z = Z ? (double)Z[at] : 8.0, s = f->f16 ? f16_value(S[at]) : (double)orc_bf2f(S[at]);
+        double t = 0.0;
+        for (uint32_t k = g * f->G; k < (g + 1u) * f->G; k++) {
+            const uint8_t b = W[(size_t)n * (f->K / 2u) + k / 2u];
+            t += ((double)((k & 1u) ? b >> 4 : b & 15u) - z) * (double)orc_bf2f(a[k]);
+        }
+        acc += t * s;
+    }
+    return acc;
+}
+/* 0x7001: t0=out t1=x t2=W t3=S t4=Z?  i0=M i1=N i2=K i3=group field i4=x pitch i5=out pitch i6=f32 out */
+static void op_gemm_w4(const PlowDevInst* in, uint32_t slice, uint32_t nblk, void* const* T) {
+    const uint32_t M = in->i[0], N = in->i[1];
+    const W4Fmt f = w4_fmt(in->i[2], in->i[3]);
+    const size_t ldx = in->i[4] ? in->i[4] : f.K, ldo = in->i[5] ? in->i[5] : N;
+    uint32_t lo, hi;
+    own_range(N, slice, nblk, &lo, &hi);
+    for (uint32_t m = 0; m < M; m++)
+        for (uint32_t n = lo; n < hi; n++) {
+            const float v = (float)w4_dot(&f, TEN(in, T, 2), TEN(in, T, 3), TEN(in, T, 4), n, (const orc_bf16*)TEN(in, T, 1) + m * ldx);
+            if (in->i[6]) ((float*)TEN(in, T, 0))[m * ldo + n] = v;
+            else ((orc_bf16*)TEN(in, T, 0))[m * ldo + n] = orc_f2bf(v);
+        }
+}
+/* 0x7002: t0=out t1=x t2=Wg t3=Sg t4=Zg? t5=Wu t6=Su t7=Zu?  i4=x pitch i5=act i6=out pitch */
+static void op_gemm_glu_w4(const PlowDevInst* in, uint32_t slice, uint32_t nblk, void* const* T) {
+    const uint32_t M = in->i[0], N = in->i[1];
+    const W4Fmt f = w4_fmt(in->i[2], in->i[3]);
+    const size_t ldx = in->i[4] ? in->i[4] : f.K, ldo = in->i[6] ? in->i[6] : N;
+    uint32_t lo, hi;
+    own_range(N, slice, nblk, &lo, &hi);
+    for (uint32_t m = 0; m < M; m++)
+        for (uint32_t n = lo; n < hi; n++) {
+            const orc_bf16* a = (const orc_bf16*)TEN(in, T, 1) + m * ldx;
+            const float g = (float)w4_dot(&f, TEN(in, T, 2), TEN(in, T, 3), TEN(in, T, 4), n, a);
+            const float u = (float)w4_dot(&f, TEN(in, T, 5), TEN(in, T, 6), TEN(in, T, 7), n, a);
+            ((orc_bf16*)TEN(in, T, 0))[m * ldo + n] = orc_f2bf(glu_pair(g, u, in->i[5], in->fj[0].f, in->fj[1].f));
+        }
+}
+static const void* tab_ptr(const uint64_t* tab, uint32_t e, uint32_t col) { return tab ? (const void*)(uintptr_t)tab[(size_t)e * 3u + col] : NULL; }
+/* expert e has what its stream `col` needs */
+static int w4_resident(const uint64_t* wtab, const uint64_t* stab, const uint64_t* ztab, uint32_t e, uint32_t col) {
+    return tab_ptr(wtab, e, col) && tab_ptr(stab, e, col) && (!ztab || tab_ptr(ztab, e, col));
+}
+/* 48 / 49 at enc 16: t3=wtab t4=stab t5=ztab?  i7=group field */
+static void op_w4_slots(const PlowDevInst* in, uint32_t slice, uint32_t nblk, void* const* T, int is_glu) {
+    const PlowMoeRoute* tab = TEN(in, T, 2);
+    const uint64_t *wtab = TEN(in, T, 3), *stab = TEN(in, T, 4), *ztab = TEN(in, T, 5);
+    const uint32_t nslot = in->i[0], N = in->i[1], E = in->i[3], kx = is_glu ? (in->i[4] ? in->i[4] : nslot) : 1u;
+    const W4Fmt f = w4_fmt(in->i[2], in->i[7]);
+    uint32_t lo, hi;
+    own_range(N, slice, nblk, &lo, &hi);
+    for (uint32_t s = 0; s < nslot; s++) {
+        const uint32_t e = tab[s].eid;
+        const orc_bf16* a = (const orc_bf16*)TEN(in, T, 1) + (size_t)(s / kx) * f.K;
+        const int ok = e < E && (is_glu ? w4_resident(wtab, stab, ztab, e, 0) && w4_resident(wtab, stab, ztab, e, 1) : w4_resident(wtab, stab, ztab, e, 2));
+        for (uint32_t n = lo; n < hi; n++) {
+            if (is_glu) {
+                if (!ok) continue;
+                const float g = (float)w4_dot(&f, tab_ptr(wtab, e, 0), tab_ptr(stab, e, 0), tab_ptr(ztab, e, 0), n, a);
+                const float u = (float)w4_dot(&f, tab_ptr(wtab, e, 1), tab_ptr(stab, e, 1), tab_ptr(ztab, e, 1), n, a);
+                ((orc_bf16*)TEN(in, T, 0))[(size_t)s * N + n] = orc_f2bf(glu_pair(g, u, in->i[5], in->fj[0].f, in->fj[1].f));
+            } else {
+                ((float*)TEN(in, T, 0))[(size_t)s * N + n] =
+                    ok ? (float)(tab[s].gate * w4_dot(&f, tab_ptr(wtab, e, 2), tab_ptr(stab, e, 2), tab_ptr(ztab, e, 2), n, a)) : 0.0f;
+            }
+        }
+    }
+}
+/* 85 / 86 at enc 16: t2=wtab t3=stab t4=meta, 85: t5=row_token t6=ztab?, 86: t5=ztab? t6=row_partidx t7=row_gate;
+ * i6=group field */
+static void op_w4_grouped(const PlowDevInst* in, uint32_t slice, uint32_t nblk, void* const* T, int is_glu) {
+    const uint64_t *wtab = TEN(in, T, 2), *stab = TEN(in, T, 3), *ztab = TEN(in, T, is_glu ? 6 : 5);
+    const int32_t* meta = TEN(in, T, 4);
+    const uint32_t* map = TEN(in, T, is_glu ? 5 : 6);
+    const uint32_t N = in->i[0], E = in->i[2];
+    const W4Fmt f = w4_fmt(in->i[1], in->i[6]);
+    uint32_t lo, hi;
+    own_range(N, slice, nblk, &lo, &hi);
+    for (uint32_t e = 0; e < E; e++) {
+        if (is_glu ? !w4_resident(wtab, stab, ztab, e, 0) || !w4_resident(wtab, stab, ztab, e, 1) : !w4_resident(wtab, stab, ztab, e, 2)) continue;
+        for (uint32_t r = (uint32_t)meta[e]; r < (uint32_t)(meta[e] + meta[E + e]); r++) {
+            if (map[r] == PLOW_EXPERT_UNUSED) continue;
+            const orc_bf16* a = (const orc_bf16*)TEN(in, T, 1) + (size_t)(is_glu ? map[r] : r) * f.K;
+            for (uint32_t n = lo; n < hi; n++) {
+                if (is_glu) {
+                    const float g = (float)w4_dot(&f, tab_ptr(wtab, e, 0), tab_ptr(stab, e, 0), tab_ptr(ztab, e, 0), n, a);
+                    const float u = (float)w4_dot(&f, tab_ptr(wtab, e, 1), tab_ptr(stab, e, 1), tab_ptr(ztab, e, 1), n, a);
+                    ((orc_bf16*)TEN(in, T, 0))[(size_t)r * N + n] = orc_f2bf(glu_pair(g, u, in->i[5], in->fj[0].f, in->fj[1].f));
+                } else {
+                    ((float*)TEN(in, T, 0))[(size_t)map[r] * N + n] =
+                        (float)(((const float*)TEN(in, T, 7))[r] * w4_dot(&f, tab_ptr(wtab, e, 2), tab_ptr(stab, e, 2), tab_ptr(ztab, e, 2), n, a));
+                }
+            }
+        }
+    }
+}
+/* 0x7010 (operands as in plow_moe.h). Rows are split over the slices. */
+static void op_logprob(const PlowDevInst* in, uint32_t slice, uint32_t nblk, void* const* T) {
+    const uint32_t rows = in->i[0], V = in->i[1], n = in->i[2], A = in->i[3];
+    const size_t pitch = in->i[4] ? in->i[4] : V, words = in->i[6] ? in->i[6] : ((size_t)V + 31u) / 32u;
+    const double c = in->fj[0].f == 0.0f ? 1.0 : (double)in->fj[0].f;
+    const uint32_t* mask = TEN(in, T, 7);
+    double* x = malloc((size_t)V * sizeof *x);
+    uint32_t lo, hi;
+    own_range(rows, slice, nblk, &lo, &hi);
+    for (uint32_t r = lo; r < hi; r++) {
+        double m = -INFINITY, z = 0.0, t = 0.0;
+        int bad = 0;
+        for (uint32_t i = 0; i < V; i++) {
+            const int ok = !mask || ((mask[r * words + i / 32u] >> (i % 32u)) & 1u);
+            x[i] = !ok ? -INFINITY : (in->i[5] & PLOW_LOGPROB_F32) ? (double)((const float*)TEN(in, T, 1))[r * pitch + i]
+                                                                   : (double)orc_bf2f(((const orc_bf16*)TEN(in, T, 1))[r * pitch + i]);
+            if (isnan(x[i]) || x[i] == INFINITY) bad = 1;
+            if (x[i] > m) m = x[i];
+        }
+        if (m == -INFINITY) m = 0.0;
+        for (uint32_t i = 0; i < V && !bad; i++) {
+            if (x[i] == -INFINITY) continue;
+            const double d = c * (x[i] - m), e = exp(d);
+            z += e;
+            t += e > 0.0 ? e * d : 0.0;
+        }
+        const double logz = bad ? NAN : log(z);
+        if (TEN(in, T, 3)) ((float*)TEN(in, T, 3))[r] = (float)(bad ? NAN : z > 0.0 ? logz - t / z : 0.0);
+        if (TEN(in, T, 6)) ((float*)TEN(in, T, 6))[r] = (float)(bad ? NAN : c * m + logz);
+        for (uint32_t j = 0; j < n; j++) {
+            const uint32_t id = ((const uint32_t*)TEN(in, T, 2))[(size_t)r * n + j];
+            ((float*)TEN(in, T, 0))[(size_t)r * n + j] =
+                id == PLOW_EXPERT_UNUSED ? 0.0f : id >= V || bad ? NAN : x[id] == -INFINITY ? -INFINITY : (float)(c * (x[id] - m) - logz);
+        }
+        /* the best not yet taken, A times: NaN first, then by value, lowest id first */
+        uint32_t* ids = TEN(in, T, 4);
+        float* lps = TEN(in, T, 5);
+        for (uint32_t a = 0; a < A; a++) {
+            uint32_t best = PLOW_EXPERT_UNUSED;
+            for (uint32_t i = 0; i < V; i++)
+                if (x[i] != -INFINITY && (best == PLOW_EXPERT_UNUSED || (isnan(x[i]) && !isnan(x[best])) || x[i] > x[best])) best = i;
+            if (ids) ids[(size_t)r * A + a] = best;
+            if (lps) lps[(size_t)r * A + a] = bad ? NAN : best == PLOW_EXPERT_UNUSED ? -INFINITY : (float)(c * (x[best] - m) - logz);
+            if (best != PLOW_EXPERT_UNUSED) x[best] = -INFINITY;
+        }
+    }
+    free(x);
+}
+
 /* ---- dispatch ---------------------------------------------------------------------------------- */
 
 typedef void (*op_fn)(const PlowDevInst*, uint32_t, uint32_t, void* const*);
@@ -1439,6 +1612,9 @@ static op_fn resolve(uint16_t op) {
     case PLOW_DOP_MOE_GLU_FP8_BLOCK128: return op_glu_fp8_block128;
     case PLOW_DOP_MOE_QUANT_FP8_BLOCK128: return op_moe_quant_block128;
     case PLOW_DOP_MOE_DOWN_FP8_BLOCK128: return op_moe_down_block128;
+    case PLOW_DOP_X_GEMM_W4: return op_gemm_w4;
+    case PLOW_DOP_X_GEMM_GLU_W4: return op_gemm_glu_w4;
+    case PLOW_DOP_X_LOGPROB: return op_logprob;
     default: return NULL;
     }
 }

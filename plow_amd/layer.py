@@ -31,12 +31,16 @@ class MoeConfig:
     n_group: int = 1
     topk_group: int = 1
     route_scale: float = 1.0
-    enc: str = "fp8blk"             # "bf16" | "fp8blk" | "mxfp4" | "fp8pc" (per-channel)
+    enc: str = "fp8blk"             # "bf16" | "fp8blk" | "mxfp4" | "fp8pc" (per-channel) | "int4g" (4-bit integers with
+                                    # group scales, arms "a16" and "a16dec"; a dense shared expert is int4 too)
     arm: str = "w8a8"               # "a16" (bf16 activations) | "w8a8" | "w8a8q" (block-fp8 only: the GLU
                                     # quantizes the bf16 rows itself, plow's arm 6; no quantizer op) |
                                     # "w8a8atomic" (block-fp8 only: ops 184, 188, 189, 190 - bf16
                                     # intermediate, slot-major quantized copy, bf16 atomic reduction into
                                     # the output; no combine op, no residual / dense shared expert)
+    group: int = 128                # int4g: columns per scale (32, 64, 128)
+    zero_points: bool = False       # int4g: stored zero points instead of 8 everywhere
+    scale_f16: bool = False         # int4g: f16 scales instead of bf16
     n_shared: int = 0
     shared_mode: Optional[str] = None  # "fold" (slot {E, 1.0}) | "dense" (ops 20 + 8) | None
     act: int = abi.ACT_SILU
@@ -53,6 +57,10 @@ class MoeConfig:
     @property
     def tail(self) -> int:
         return 1 if self.shared_mode == "fold" else 0
+
+    @property
+    def group_field(self) -> int:
+        return self.group | (abi.W4_SCALE_F16 if self.scale_f16 else 0)
 
     @property
     def E_all(self) -> int:      # experts the align / grouped ops see
@@ -100,6 +108,11 @@ def config(name: str, T: Optional[int] = None) -> MoeConfig:
     if name == "c5":   # Qwen3-MoE-shaped per-channel fp8, no shared expert
         return MoeConfig("c5", H=4096, E=128, I=1536, k=8, T=T or 64, scoring="softmax",
                          norm_topk=True, enc="fp8pc", arm="a16")
+    if name == "c7":   # Kimi-K2-shaped, 4-bit integers with a scale per 32 columns
+        T = T or 16
+        return MoeConfig("c7", H=7168, E=384, I=2048, k=8, T=T, scoring="sigmoid", norm_topk=True, bias=True,
+                         route_scale=2.827, enc="int4g", group=32, n_shared=1, shared_mode="fold",
+                         arm="a16dec" if T * 9 <= 128 else "a16", emit_align=T * 9 > 128)
     if name == "c6":   # GLM-5.3-Flash-shaped block-fp8, one rank's slice of TP8 (the shape of plow's
         # own gfx950 prefill bench, runtime/bench/amd/moe_fp8_pf_bench.hip:1-7)
         return MoeConfig("c6", H=4096, E=288, I=256, k=8, T=T or 8192, scoring="sigmoid",
@@ -109,7 +122,7 @@ def config(name: str, T: Optional[int] = None) -> MoeConfig:
 
 @dataclass
 class TensorSpec:
-    dtype: str                 # "bf16" "f32" "u8" "i32" "u32" "u64" "route"
+    dtype: str                 # "bf16" "f16" "f32" "u8" "i32" "u32" "u64" "route"
     shape: Tuple[int, ...]
     role: str                  # "in" | "weight" | "scratch" | "out" | "table"
 
@@ -127,6 +140,12 @@ class LayerPlan:
             self.slots[name] = len(self.slots)
             self.specs[name] = TensorSpec(dtype, tuple(int(s) for s in shape), role)
         return self.slots[name]
+
+    def _int4(self, name: str, N: int, K: int, cfg) -> List[Optional[int]]:
+        """Slots of one int4 tensor: packed weights, scales, zero points (None: 8 everywhere)."""
+        return [self._t(name, "u8", (N, K // 2), "weight"),
+                self._t(name + "_scale", "f16" if cfg.scale_f16 else "bf16", (N, K // cfg.group), "weight"),
+                self._t(name + "_zero", "u8", (N, K // cfg.group), "weight") if cfg.zero_points else None]
 
     def _emit(self, label: str, d: abi.PlowDevInst):
         self.insts.append(d)
@@ -202,16 +221,20 @@ def plan_layer(cfg: MoeConfig, with_router_score: bool = True) -> LayerPlan:
             p._emit("down", abi.inst(abi.OP_MOE_EXPERT_DOWN_GEMMA_FP8, t=[part, fu, table, ewt, est],
                                      i=[ka, H, I, Ea, 0, T]))
     else:
-        enc = {"bf16": abi.ENC_BF16, "fp8blk": abi.ENC_FP8BLK, "mxfp4": abi.ENC_MXFP4}[cfg.enc]
+        enc = {"bf16": abi.ENC_BF16, "fp8blk": abi.ENC_FP8BLK, "mxfp4": abi.ENC_MXFP4, "int4g": abi.ENC_INT4G}[cfg.enc]
+        int4 = enc == abi.ENC_INT4G
+        assert not int4 or cfg.arm in ("a16", "a16dec"), "int4 weights take bf16 activations"
+        ztab = p._t("ztab", "u64", (Ea, 3), "table") if int4 and cfg.zero_points else None
+        gf = cfg.group_field if int4 else 0
         wtab = p._t("wtab", "u64", (Ea, 3), "table")
         stab = p._t("stab", "u64", (Ea, 3), "table") if enc != abi.ENC_BF16 else None
         if cfg.arm == "a16dec":
             # plow's decode experts (ops 48 / 49): bf16 activations, table driven, slot-major rows, no op 84
             fu = p._t("fu", "bf16", (T * ka, I), "scratch")
-            p._emit("glu", abi.inst(abi.OP_MOE_GROUP_GLU_FP8_BLK, t=[fu, x, table, wtab, stab],
-                                    i=[T * ka, I, H, Ea, ka, cfg.act, enc]))
-            p._emit("down", abi.inst(abi.OP_MOE_GROUP_DOWN_FP8_BLK, t=[part, fu, table, wtab, stab],
-                                     i=[T * ka, H, I, Ea, 0, 0, enc]))
+            p._emit("glu", abi.inst(abi.OP_MOE_GROUP_GLU_FP8_BLK, t=[fu, x, table, wtab, stab, ztab],
+                                    i=[T * ka, I, H, Ea, ka, cfg.act, enc, gf], f=cfg.act_f if int4 else ()))
+            p._emit("down", abi.inst(abi.OP_MOE_GROUP_DOWN_FP8_BLK, t=[part, fu, table, wtab, stab, ztab],
+                                     i=[T * ka, H, I, Ea, 0, 0, enc, gf]))
         elif enc == abi.ENC_FP8BLK and cfg.arm == "w8a8atomic":
             assert cfg.shared_mode != "dense" and not cfg.residual, "the atomic chain has no combine op"
             xq = p._t("xq", "u8", (T, H), "scratch")
@@ -271,15 +294,23 @@ def plan_layer(cfg: MoeConfig, with_router_score: bool = True) -> LayerPlan:
             arm = abi.ARM_W4A16 if enc == abi.ENC_MXFP4 else abi.ARM_A16
             fu = p._t("fu", "bf16", (R, I), "scratch")
             p._emit("glu", abi.inst(abi.OP_MOE_GROUP_GLU_PF,
-                                    t=[fu, x, wtab, stab, meta, row_token],
-                                    i=[I, H, Ea, enc, 0, cfg.act, 0, arm], f=cfg.act_f, slots=T * ka))
+                                    t=[fu, x, wtab, stab, meta, row_token, ztab],
+                                    i=[I, H, Ea, enc, 0, cfg.act, gf, arm], f=cfg.act_f, slots=T * ka))
             p._emit("down", abi.inst(abi.OP_MOE_GROUP_DOWN_PF,
-                                     t=[part, fu, wtab, stab, meta, None, row_partidx, row_gate],
-                                     i=[H, I, Ea, enc, 0, 0, 0, arm], slots=T * ka))
+                                     t=[part, fu, wtab, stab, meta, ztab, row_partidx, row_gate],
+                                     i=[H, I, Ea, enc, 0, 0, gf, arm], slots=T * ka))
 
     shared = None
     if cfg.shared_mode == "dense":
         Is = cfg.I_shared
+    if cfg.shared_mode == "dense" and cfg.enc == "int4g":
+        gate, up, down = (p._int4(f"Ws_{n}", a, b, cfg) for n, a, b in (("gate", Is, H), ("up", Is, H), ("down", H, Is)))
+        sfu = p._t("shared_fu", "bf16", (T, Is), "scratch")
+        shared = p._t("shared", "bf16", (T, H), "scratch")
+        p._emit("shared_glu", abi.inst(abi.OP_X_GEMM_GLU_W4, t=[sfu, x, *gate, *up],
+                                       i=[T, Is, H, cfg.group_field, 0, cfg.act], f=cfg.act_f))
+        p._emit("shared_down", abi.inst(abi.OP_X_GEMM_W4, t=[shared, sfu, *down], i=[T, H, Is, cfg.group_field]))
+    elif cfg.shared_mode == "dense":
         wsg = p._t("Ws_gate", "bf16", (Is, H), "weight")
         wsu = p._t("Ws_up", "bf16", (Is, H), "weight")
         wsd = p._t("Ws_down", "bf16", (H, Is), "weight")
@@ -290,4 +321,52 @@ def plan_layer(cfg: MoeConfig, with_router_score: bool = True) -> LayerPlan:
         p._emit("shared_down", abi.inst(abi.OP_GEMM, t=[shared, sfu, wsd], i=[T, H, Is]))
     p._emit("combine", abi.inst(abi.OP_MOE_COMBINE_PF, t=[out, residual, shared, part],
                                 i=[H, 1 if det else ka, T, 0, 1 if det else 0, 0, 0, 1 if p16 else 0]))
+    return p
+
+
+@dataclass
+class HeadConfig:
+    """The end of a model: final norm, logits over the vocabulary, log probabilities."""
+    name: str
+    T: int
+    H: int
+    V: int
+    enc: str = "bf16"               # "bf16" (op 180) | "int4g"
+    group: int = 128
+    zero_points: bool = False
+    scale_f16: bool = False
+    n_given: int = 1                # given tokens per row whose log probability is asked for
+    n_alt: int = 0                  # most likely tokens per row
+    entropy: bool = True
+    masked: bool = False            # a bit mask of allowed tokens per row
+    scale: float = 1.0              # multiplies the logits (1 / temperature)
+    eps: float = 1e-6
+
+    @property
+    def group_field(self) -> int:
+        return self.group | (abi.W4_SCALE_F16 if self.scale_f16 else 0)
+
+
+def plan_head(cfg: HeadConfig) -> LayerPlan:
+    """Emit the chain RMSNorm (1) -> logits (180, or the int4 product) -> log probabilities (0x7010)."""
+    p = LayerPlan(cfg)
+    T, H, V = cfg.T, cfg.H, cfg.V
+    x = p._t("x", "bf16", (T, H), "in")
+    gamma = p._t("gamma", "bf16", (H,), "weight")
+    xn = p._t("xn", "bf16", (T, H), "scratch")
+    logits = p._t("logits", "f32", (T, V), "scratch")
+    p._emit("norm", abi.inst(abi.OP_RMSNORM, t=[xn, x, gamma], i=[T, H], f=[cfg.eps]))
+    if cfg.enc == "int4g":
+        p._emit("logits", abi.inst(abi.OP_X_GEMM_W4, t=[logits, xn, *p._int4("Wh", V, H, cfg)],
+                                   i=[T, V, H, cfg.group_field, 0, 0, 1]))
+    else:
+        p._emit("logits", abi.inst(abi.OP_GEMM_F32, t=[logits, xn, p._t("Wh", "bf16", (V, H), "weight")], i=[T, V, H]))
+    n, A = cfg.n_given, cfg.n_alt
+    given = (p._t("logprob", "f32", (T, n), "out"), p._t("tokens", "u32", (T, n), "in")) if n else (None, None)
+    p._emit("logprob", abi.inst(
+        abi.OP_X_LOGPROB,
+        t=[given[0], logits, given[1], p._t("entropy", "f32", (T,), "out") if cfg.entropy else None,
+           p._t("alt_tokens", "u32", (T, A), "out") if A else None, p._t("alt_logprob", "f32", (T, A), "out") if A else None,
+           p._t("lse", "f32", (T,), "out"), p._t("allowed", "u32", (T, (V + 31) // 32), "in") if cfg.masked else None],
+        i=[T, V, n, A, 0, abi.LOGPROB_F32], f=[cfg.scale]))
     return p

@@ -9,6 +9,7 @@ definition: activations ~N(0,1), expert / shared / router weights ~N(0,0.02), ro
               (DeepSeek ``weight_scale_inv`` convention; layout runtime/common/dev_isa.h:442-445)
   per-channel e4m3 with one f32 scale per output row, scale = amax_row / 448
               (perf-data/tools/quantize_fp8.py:204-207)
+  int4g       4-bit integers, one bf16 / f16 scale per group of 32, 64 or 128 columns, optional zero points
   mxfp4       e2m1 + E8M0 per 32: scale 2^e with amax / 2^e in (3, 6], round to nearest with ties
               toward zero, all-zero block -> 2^-3 (perf-data/tools/quantize_mxfp4.py:38-55)
 
@@ -23,7 +24,7 @@ import torch
 from . import abi
 from .layer import LayerPlan, MoeConfig
 
-_TORCH_DT = {"bf16": torch.bfloat16, "f32": torch.float32, "f64": torch.float64, "u8": torch.uint8,
+_TORCH_DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32, "f64": torch.float64, "u8": torch.uint8,
              "i32": torch.int32, "u32": torch.int32, "u64": torch.int64}
 
 E4M3_MAX = 448.0
@@ -79,6 +80,26 @@ def quant_mxfp4(w: torch.Tensor):
     return packed.contiguous(), (e + 127).to(torch.uint8).contiguous()
 
 
+def quant_int4_group(w: torch.Tensor, group: int, zero_points: bool = False, scale_f16: bool = False):
+    """w [N, K] -> (packed u8 [N, K/2] low nibble = even k, scales bf16 | f16 [N, K/group], zero points u8 or None).
+    Symmetric: scale amax / 7, codes round(w / scale) + 8 in 1..15; with zero points: scale (max - min) / 15 over a
+    range that holds 0, code and zero point in 0..15. Codes are taken with the scale as stored."""
+    N, K = w.shape
+    blk = w.float().view(N, K // group, group)
+    dt = torch.float16 if scale_f16 else torch.bfloat16
+    if zero_points:
+        lo, hi = blk.amin(2).clamp(max=0.0), blk.amax(2).clamp(min=0.0)
+        scale = torch.where(hi > lo, (hi - lo) / 15.0, torch.ones_like(hi)).to(dt)
+        zero = (-lo / scale.float()).round().clamp(0, 15)
+    else:
+        amax = blk.abs().amax(2)
+        scale = torch.where(amax > 0, amax / 7.0, torch.ones_like(amax)).to(dt)
+        zero = torch.full_like(amax, 8.0)
+    q = ((blk / scale.float().unsqueeze(2)).round() + zero.unsqueeze(2)).clamp(0, 15).to(torch.uint8).view(N, K)
+    packed = (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous()
+    return packed, scale.contiguous(), zero.to(torch.uint8).contiguous() if zero_points else None
+
+
 class Bound:
     """Tensors of one plan on one device plus the handle table pointing at them."""
 
@@ -86,6 +107,7 @@ class Bound:
         self.plan, self.device = plan, torch.device(device)
         self.t: Dict[str, torch.Tensor] = {}
         self.experts = []          # keeps the per-expert weight tensors alive
+        self.zeros = []            # int4g with zero points: per expert set (gate, up, down)
         self._table = None
 
     def alloc(self, name: str, fill: Optional[float] = None) -> torch.Tensor:
@@ -99,6 +121,14 @@ class Bound:
         self.t[name] = t
         self._table = None
         return t
+
+    def set_int4(self, name: str, w: torch.Tensor):
+        """Quantize ``w`` into the plan's int4 tensor ``name`` (its scales and zero points with it)."""
+        cfg = self.plan.cfg
+        self.t[name], self.t[name + "_scale"], z = quant_int4_group(w, cfg.group, cfg.zero_points, cfg.scale_f16)
+        if z is not None:
+            self.t[name + "_zero"] = z
+        self._table = None
 
     def table(self):
         """ctypes ``void*[]`` handle table (device or host pointers, by where the tensors live)."""
@@ -114,7 +144,7 @@ class Bound:
         """Host copy of a tensor as a numpy array (bf16 as its uint16 bits; routes as (eid, gate))."""
         t = self.t[name].detach().cpu().contiguous()
         sp = self.plan.specs[name]
-        if sp.dtype == "bf16":
+        if sp.dtype in ("bf16", "f16"):
             return t.view(torch.int16).numpy().view(np.uint16)
         if sp.dtype == "u32":
             return t.numpy().view(np.uint32)
@@ -173,7 +203,10 @@ def bind(plan: LayerPlan, device, seed: int = 0, x_std: float = 1.0, w_std: floa
                        else torch.randn(cfg.E, generator=_gen(dev, seed * 1000 + 3), device=dev) * 0.01)
     if cfg.residual:
         b.t["residual"] = randn_bf16((cfg.T, cfg.H), x_std, dev, seed * 1000 + 4)
-    if cfg.shared_mode == "dense":
+    if cfg.shared_mode == "dense" and cfg.enc == "int4g":
+        for n, (name, rows, cols) in enumerate((("gate", cfg.I_shared, cfg.H), ("up", cfg.I_shared, cfg.H), ("down", cfg.H, cfg.I_shared))):
+            b.set_int4("Ws_" + name, randn_bf16((rows, cols), w_std, dev, seed * 1000 + 5 + n))
+    elif cfg.shared_mode == "dense":
         Is = cfg.I_shared
         b.t["Ws_gate"] = randn_bf16((Is, cfg.H), w_std, dev, seed * 1000 + 5)
         b.t["Ws_up"] = randn_bf16((Is, cfg.H), w_std, dev, seed * 1000 + 6)
@@ -182,7 +215,9 @@ def bind(plan: LayerPlan, device, seed: int = 0, x_std: float = 1.0, w_std: floa
     Ea = cfg.E_all
     wname, sname = ("ewt", "est") if cfg.enc == "fp8pc" else ("wtab", "stab")
     if share is not None:
-        b.experts = share.experts
+        b.experts, b.zeros = share.experts, share.zeros
+        if "ztab" in plan.slots:
+            b.t["ztab"] = share.t["ztab"]
         b.t[wname] = share.t[wname]
         if sname in plan.slots:
             b.t[sname] = share.t[sname]
@@ -203,6 +238,11 @@ def bind(plan: LayerPlan, device, seed: int = 0, x_std: float = 1.0, w_std: floa
         elif cfg.enc == "mxfp4":
             q = [quant_mxfp4(w) for w in (g, u, d)]
             sets.append((tuple(a for a, _ in q), tuple(s for _, s in q)))
+        elif cfg.enc == "int4g":
+            q = [quant_int4_group(w, cfg.group, cfg.zero_points, cfg.scale_f16) for w in (g, u, d)]
+            sets.append((tuple(a for a, _, _ in q), tuple(s for _, s, _ in q)))
+            if cfg.zero_points:
+                b.zeros.append(tuple(z for _, _, z in q))
         elif cfg.enc == "fp8pc":
             gu = torch.cat([g, u], dim=0)
             (qgu, sgu), (qd, sd) = quant_fp8_channel(gu), quant_fp8_channel(d)
@@ -222,6 +262,33 @@ def bind(plan: LayerPlan, device, seed: int = 0, x_std: float = 1.0, w_std: floa
     b.t[wname] = wt.to(dev)
     if sname in plan.slots:
         b.t[sname] = st.to(dev)
+    if "ztab" in plan.slots:
+        b.t["ztab"] = torch.tensor([[z.data_ptr() for z in b.zeros[e % n_distinct]] for e in range(Ea)], dtype=torch.int64).to(dev)
+    b._table = None
+    return b
+
+
+def bind_head(plan: LayerPlan, device, seed: int = 0, x_std: float = 1.0, w_std: float = 0.02) -> Bound:
+    """Allocate and fill every tensor of a head plan (``layer.plan_head``): random rows, norm weights around 1, a
+    random output matrix, given tokens and, where the plan has one, a mask that allows about half of the tokens."""
+    cfg = plan.cfg
+    b = Bound(plan, device)
+    dev = b.device
+    for name in plan.specs:
+        if plan.specs[name].role in ("scratch", "out"):
+            b.alloc(name)
+    b.t["x"] = randn_bf16((cfg.T, cfg.H), x_std, dev, seed * 1000 + 1)
+    b.t["gamma"] = (1.0 + 0.1 * torch.randn(cfg.H, generator=_gen(dev, seed * 1000 + 2), device=dev)).to(torch.bfloat16)
+    w = randn_bf16((cfg.V, cfg.H), w_std, dev, seed * 1000 + 3)
+    if cfg.enc == "int4g":
+        b.set_int4("Wh", w)
+    else:
+        b.t["Wh"] = w
+    if cfg.n_given:
+        b.t["tokens"] = torch.randint(0, cfg.V, (cfg.T, cfg.n_given), generator=_gen(dev, seed * 1000 + 4), device=dev, dtype=torch.int32)
+    if cfg.masked:
+        b.t["allowed"] = torch.randint(-2 ** 31, 2 ** 31, (cfg.T, (cfg.V + 31) // 32), generator=_gen(dev, seed * 1000 + 5),
+                                       device=dev, dtype=torch.int64).to(torch.int32)
     b._table = None
     return b
 
@@ -231,10 +298,13 @@ def to_host(b: Bound) -> Bound:
     plan = b.plan
     h = Bound(plan, "cpu")
     for name, t in b.t.items():
-        if name not in ("wtab", "stab", "ewt", "est"):
+        if name not in ("wtab", "stab", "ztab", "ewt", "est"):
             h.t[name] = t.detach().cpu().clone()
+    if not b.experts:          # a head: no expert tables
+        return h
     h.experts = [(tuple(w.cpu() for w in ws), tuple(None if s is None else s.cpu() for s in ss))
                  for ws, ss in b.experts]
+    h.zeros = [tuple(z.cpu() for z in zs) for zs in b.zeros]
     cfg = plan.cfg
     wname, sname = ("ewt", "est") if cfg.enc == "fp8pc" else ("wtab", "stab")
     width = 2 if cfg.enc == "fp8pc" else 3
@@ -249,4 +319,6 @@ def to_host(b: Bound) -> Bound:
     h.t[wname] = wt
     if sname in plan.slots:
         h.t[sname] = st
+    if "ztab" in plan.slots:
+        h.t["ztab"] = torch.tensor([[z.data_ptr() for z in h.zeros[e % nd]] for e in range(cfg.E_all)], dtype=torch.int64)
     return h
