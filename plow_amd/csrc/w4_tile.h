@@ -17,7 +17,7 @@
  * if G = 128. For G = 64 two and for G = 32 four cross-lane swaps per 16 bytes re-deal the dwords so that instruction r
  * covers columns of one group; w4_koff says which, and the x operand is read accordingly.
  *
- * Staging. Weights and x of the next D steps are on their way in registers (plain loads, whole 64- or 128-byte runs
+ * Staging. Weights and x of the next step are on their way in registers (plain loads, whole 64- or 256-byte runs
  * per row); a step is written to one of two LDS buffers, one barrier per step that orders LDS only. Scales and zero
  * points come CC columns at a time, in runs of up to 64 bytes per row: read step by step, a few bytes of a line each,
  * they cost as many requests as the weights themselves. What lies behind K, behind the last row or the last channel is staged as zero, so that every step runs whole. */
@@ -36,6 +36,7 @@ struct W4Tiles {
 };
 
 __device__ __forceinline__ float w4_f32(uint32_t h, uint32_t f16) {
+    asm("" : "+v"(f16)); /* a select, no branch */
     return f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : __uint_as_float(h << 16);
 }
 
@@ -107,9 +108,9 @@ __device__ __forceinline__ float w4_run_sum(float v) {
 }
 
 /* CC: columns whose scales are staged together (a multiple of KS) */
-template <int WT_, int WC_, int MTW_, int NBW_, int NS_, int KS_, int D_, int CC_, int G_, bool ASYM_>
+template <int WT_, int WC_, int MTW_, int NBW_, int NS_, int KS_, int CC_, int G_, bool ASYM_>
 struct W4Cfg {
-    static constexpr int WT = WT_, WC = WC_, MTW = MTW_, NBW = NBW_, NS = NS_, KS = KS_, D = D_, CC = CC_, G = G_;
+    static constexpr int WT = WT_, WC = WC_, MTW = MTW_, NBW = NBW_, NS = NS_, KS = KS_, CC = CC_, G = G_;
     static constexpr bool ASYM = ASYM_;
     static constexpr int THREADS = WT * WC * 64, TM = WT * MTW * 16, TN = WC * NBW * 16;
     static constexpr int GS = KS / G;                      /* groups per step */
@@ -130,6 +131,7 @@ struct W4Cfg {
     static_assert(LDS <= 160 * 1024, "two buffers fit the CU");
     static_assert(CC % KS == 0 && CC % 128 == 0 && SP >= 4 && ZP >= 4, "a chunk is whole steps");
     static_assert(THREADS % XP == 0 && XP % (G / 8) == 0, "a group's pieces lie in neighbouring lanes");
+    static_assert(TN % (THREADS / WP) == 0 && XL % (G / 8 < XL ? G / 8 : XL) == 0, "a load covers rows of one stream");
 };
 
 /* what a thread has on its way for one step, and for one chunk's scales */
@@ -156,30 +158,37 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
 
     /* ---- where this thread's pieces come from ---- */
     const uint8_t* xsrc[C::XL];
-    bool xok[C::XL];
     const uint32_t xp = tid % C::XP;
 #pragma unroll
     for (int j = 0; j < C::XL; j++) {
         const uint32_t t = rb + (tid + (uint32_t)j * C::THREADS) / C::XP;
         uint32_t ai = PLOW_EXPERT_UNUSED;
         if (t < cnt) ai = g.a_idx ? g.a_idx[r0 + t] : r0 + t;
-        xok[j] = ai != PLOW_EXPERT_UNUSED;
-        xsrc[j] = (const uint8_t*)g.x + ((size_t)(xok[j] ? ai : 0u) * g.ldx + xp * 8u) * 2u;
+        xsrc[j] = (const uint8_t*)g.x + (size_t)(ai != PLOW_EXPERT_UNUSED ? ai : 0u) * g.ldx * 2u;
     }
-    auto tensor = [&](const uint64_t* tab, const void* const* direct, uint32_t st) -> const uint8_t* {
-        return g.wtab ? (tab ? (const uint8_t*)(uintptr_t)tab[(size_t)e * 3u + g.sel[st]] : nullptr) : (const uint8_t*)direct[st];
+    /* a tile's first channel of each stream, and 32-bit offsets from there (K < 2^24, so they fit) */
+    auto tensor = [&](const uint64_t* tab, const void* const* direct, uint32_t st, uint32_t pitch) -> const uint8_t* {
+        const uint8_t* const p = tab ? (const uint8_t*)(uintptr_t)tab[(size_t)e * 3u + g.sel[st]] : (const uint8_t*)direct[st];
+        return p + (size_t)n0 * pitch;
     };
-    const uint8_t* wsrc[C::WL];
-    const uint32_t wp = tid % C::WP;
+    const uint8_t *wbase[NS], *sbase[NS], *zbase[NS];
+#pragma unroll
+    for (int st = 0; st < NS; st++) {
+        wbase[st] = tensor(g.wtab, g.w, st, K / 2u), sbase[st] = tensor(g.stab, g.s, st, KG * 2u);
+        zbase[st] = C::ASYM ? tensor(g.ztab, g.z, st, KG) : nullptr;
+    }
+    const uint32_t wp = tid % C::WP, last = N - 1u - n0;
+    constexpr int WR = C::THREADS / C::WP, XR = C::THREADS / C::XP; /* rows that the workgroup loads at once */
+    uint32_t woff[C::WL];
 #pragma unroll
     for (int j = 0; j < C::WL; j++) {
-        const uint32_t row = (tid + (uint32_t)j * C::THREADS) / C::WP, st = NS == 2 ? row / C::TN : 0u, ch = n0 + row % C::TN;
-        wsrc[j] = tensor(g.wtab, g.w, st) + (size_t)(ch < N ? ch : N - 1u) * (K / 2u) + wp * 16u;
+        const uint32_t ch = tid / C::WP + (uint32_t)(j * WR % C::TN);
+        woff[j] = (ch < last ? ch : last) * (K / 2u);
     }
     /* scale piece j of this thread: weight row (stream, channel) and the first of its SP bytes in the chunk */
-    auto scale_row = [&](const uint64_t* tab, const void* const* direct, uint32_t row, uint32_t elem) -> const uint8_t* {
-        const uint32_t st = NS == 2 ? row / C::TN : 0u, ch = n0 + row % C::TN;
-        return tensor(tab, direct, st) + (size_t)(ch < N ? ch : N - 1u) * KG * elem;
+    auto scale_row = [&](const uint8_t* const* base, uint32_t row, uint32_t pitch) -> const uint8_t* {
+        const uint32_t ch = row % C::TN;
+        return (NS == 2 && row >= (uint32_t)C::TN ? base[NS - 1] : base[0]) + (ch < last ? ch : last) * pitch;
     };
     auto load_scales = [&](W4Scales<C>& b, uint32_t step) { /* of the chunk that starts with `step` */
         const uint32_t g0 = step * C::GS;
@@ -188,7 +197,7 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
         for (int j = 0; j < C::SL; j++) {
             const uint32_t i = tid + (uint32_t)j * C::THREADS, row = i / (C::SB / C::SP), off = (i % (C::SB / C::SP)) * C::SP;
             if (C::SN % C::THREADS == 0 || i < (uint32_t)C::SN) {
-                const uint8_t* const p = scale_row(g.stab, g.s, row, 2u) + (size_t)g0 * 2u + off;
+                const uint8_t* const p = scale_row(sbase, row, KG * 2u) + g0 * 2u + off;
                 if (whole) {
                     __builtin_memcpy(b.s[j], p, C::SP); /* rows are aligned to an element only */
                 } else {
@@ -206,7 +215,7 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
         for (int j = 0; j < C::ZL; j++) {
             const uint32_t i = tid + (uint32_t)j * C::THREADS, row = i / (C::ZB / C::ZP), off = (i % (C::ZB / C::ZP)) * C::ZP;
             if (C::ZN % C::THREADS == 0 || i < (uint32_t)C::ZN) {
-                const uint8_t* const p = scale_row(g.ztab, g.z, row, 1u) + g0 + off;
+                const uint8_t* const p = scale_row(zbase, row, KG) + g0 + off;
                 if (whole) {
                     __builtin_memcpy(b.z[j], p, C::ZP);
                 } else {
@@ -237,36 +246,58 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
         }
     };
 
+    /* No load stands under a condition, so that the compiler can count what is in flight: a step past the end is the
+     * last one again, a piece past the end of a row the row's last (x counts as zero there), a row that is not there
+     * row 0. */
     auto load = [&](W4Stage<C>& b, uint32_t step) {
-        const uint32_t k0 = step * KS;
-        const bool whole = k0 + KS <= K;
+        step = step < s_hi ? step : s_hi - 1u;
+        const uint32_t k = step * KS, wk = k / 2u + wp * 16u, xk = k + xp * 8u;
+        const uint32_t wo = wk < K / 2u - 16u ? wk : K / 2u - 16u, xo = xk < K - 8u ? xk : K - 8u;
 #pragma unroll
-        for (int j = 0; j < C::WL; j++)
-            b.w[j] = whole || k0 + wp * 32u < K ? *(const v4i*)(wsrc[j] + (size_t)step * (KS / 2)) : (v4i){0, 0, 0, 0};
+        for (int j = 0; j < C::WL; j++) b.w[j] = *(const v4i*)(wbase[j * WR / C::TN] + (woff[j] + wo));
 #pragma unroll
-        for (int j = 0; j < C::XL; j++)
-            b.x[j] = xok[j] && (whole || k0 + xp * 8u < K) ? *(const v4i*)(xsrc[j] + (size_t)step * (KS * 2)) : (v4i){0, 0, 0, 0};
+        for (int j = 0; j < C::XL; j++) b.x[j] = *(const v4i*)(xsrc[j] + (size_t)xo * 2u);
     };
+    /* rows that are not there hold some other row: nothing of them is stored */
+    const uint32_t wst = (tid / C::WP) * C::WROW + wp * 16u, xst = (tid / C::XP) * C::XROW + xp * 16u;
     auto stage = [&](const W4Stage<C>& b, uint8_t* buf) {
         uint8_t* const xl = buf;
         uint8_t* const wl = buf + C::X_BYTES;
         float* const xs = (float*)(buf + C::X_BYTES + C::W_BYTES);
+        typedef float __attribute__((ext_vector_type(C::XL))) xsum_t; /* (an array's selects become scratch memory) */
+        xsum_t xsum = {};
 #pragma unroll
-        for (int j = 0; j < C::WL; j++) *(v4i*)(wl + ((tid + j * C::THREADS) / C::WP) * C::WROW + wp * 16u) = b.w[j];
+        for (int j = 0; j < C::WL; j++)
+            *(v4i*)(wl + wst + j * WR * C::WROW) = b.w[j];
 #pragma unroll
         for (int j = 0; j < C::XL; j++) {
-            const uint32_t t = (tid + j * C::THREADS) / C::XP;
-            *(v4i*)(xl + t * C::XROW + xp * 16u) = w4_order(b.x[j]);
+            *(v4i*)(xl + xst + j * XR * C::XROW) = w4_order(b.x[j]);
             float v = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; i++) v = w4_dot2((uint32_t)b.x[j][i], 0x3F803F80u, v);
-            v = w4_run_sum<G / 8>(v);
-            if (xp % (G / 8) == 0u) xs[(xp / (G / 8)) * C::TM + t] = C::ASYM ? -v : -24.0f * v;
+            xsum[j] = w4_run_sum<G / 8>(v);
         }
+        /* the lanes of a group's run hold the same sum: lane j of the run stores that of row j */
+        constexpr int RUN = G / 8 < C::XL ? G / 8 : C::XL;
+#pragma unroll
+        for (int j0 = 0; j0 < C::XL; j0 += RUN) {
+            float v = xsum[j0];
+            uint32_t mine = xp % (G / 8);
+#pragma unroll
+            for (int j = 1; j < RUN; j++) v = mine == (uint32_t)j ? xsum[j0 + j] : v;
+            if (RUN == G / 8 || mine < RUN) xs[(xp / (G / 8)) * C::TM + tid / C::XP + (j0 + mine) * XR] = C::ASYM ? -v : -24.0f * v;
+        }
+    };
+    /* columns behind K count as zero; the walk calls this for the step that has some */
+    auto cut = [&](W4Stage<C>& b, uint32_t step) {
+        if (step * KS + xp * 8u < K) return;
+#pragma unroll
+        for (int j = 0; j < C::XL; j++) b.x[j] = (v4i){0, 0, 0, 0};
     };
 
     const W4Bits bits = w4_bits();
     v4f acc[NS][C::NBW][C::MTW] = {};
+    constexpr int TILES = NS * C::NBW;
     auto multiply = [&](const uint8_t* buf, const uint8_t* sbuf, uint32_t g0) { /* g0: the step's first group in its chunk */
         const uint8_t* const xl = buf + (wt * C::MTW * 16u + c) * C::XROW;
         const uint8_t* const wl = buf + C::X_BYTES;
@@ -275,16 +306,17 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
         const uint8_t* const zl = sbuf + C::S_BYTES + (wc * C::NBW * 16u + c) * C::ZROW + g0;
 #pragma unroll
         for (int blk = 0; blk < KS / 128; blk++) {
-            uint32_t raw[NS][C::NBW][4];
+            /* a lane's 32 weights of 16 channels: one group (G = 128) is read one turn ahead, several stay */
+            constexpr int RAW = G == 128 ? 2 : TILES;
+            uint32_t raw[RAW][4];
+            auto fetch = [&](int i) {
+                const v4i w = *(const v4i*)(wl + ((i / C::NBW) * C::TN + wc * C::NBW * 16u + (i % C::NBW) * 16u + c) * C::WROW + blk * 64u + q * 16u);
 #pragma unroll
-            for (int st = 0; st < NS; st++)
+                for (int k = 0; k < 4; k++) raw[i % RAW][k] = (uint32_t)w[k];
+                w4_deal<G>(raw[i % RAW]);
+            };
 #pragma unroll
-                for (int nb = 0; nb < C::NBW; nb++) {
-                    const v4i w = *(const v4i*)(wl + (st * C::TN + wc * C::NBW * 16u + nb * 16u + c) * C::WROW + blk * 64u + q * 16u);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) raw[st][nb][i] = (uint32_t)w[i];
-                    w4_deal<G>(raw[st][nb]);
-                }
+            for (int i = 0; i < (G == 128 ? 1 : TILES); i++) fetch(i);
             constexpr int RG = G / 32; /* instructions per group */
 #pragma unroll
             for (int gr = 0; gr < 128 / G; gr++) {
@@ -304,9 +336,11 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
                     for (int nb = 0; nb < C::NBW; nb++) {
                         const float s = w4_f32(*(const uint16_t*)(sl + (st * C::TN + nb * 16) * C::SROW + gi * 2), g.s_f16);
                         const float zc = C::ASYM ? 16.0f + (float)zl[(st * C::TN + nb * 16) * C::ZROW + gi] : 0.0f;
+                        const int i = st * C::NBW + nb;
+                        if (G == 128 && i + 1 < TILES) fetch(i + 1);
                         v8bf b[RG];
 #pragma unroll
-                        for (int r = 0; r < RG; r++) b[r] = w4_unpack(raw[st][nb][gr * RG + r], bits);
+                        for (int r = 0; r < RG; r++) b[r] = w4_unpack(raw[i % RAW][gr * RG + r], bits);
 #pragma unroll
                         for (int mt = 0; mt < C::MTW; mt++) {
                             v4f t = cx[mt];
@@ -319,37 +353,31 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
 #pragma unroll
                             for (int i = 0; i < 4; i++) acc[st][nb][mt][i] = fmaf(t[i], s, acc[st][nb][mt][i]);
                         }
+                        __builtin_amdgcn_sched_barrier(0); /* (more in flight at once does not fit the registers) */
                     }
             }
         }
     };
 
-    /* ---- the walk over K: D steps on their way, two LDS buffers ---- */
-    W4Stage<C> ring[C::D];
+    /* ---- the walk over K: the next step is on its way in registers, two LDS buffers ---- */
+    W4Stage<C> ring;
     W4Scales<C> sring;
-    if (s_lo < s_hi) load_scales(sring, s_lo);
-#pragma unroll
-    for (int d = 0; d < C::D; d++)
-        if (s_lo + d < s_hi) load(ring[d], s_lo + d);
-    for (uint32_t s0 = s_lo; s0 < s_hi; s0 += C::D) {
-#pragma unroll
-        for (int d = 0; d < C::D; d++) {
-            const uint32_t s = s0 + d;
-            if (s < s_hi) { /* the same in every lane */
-                const uint32_t n = s - s_lo, in_chunk = n % C::CS;
-                uint8_t* const buf = lds + (n & 1u) * C::BUF;
-                uint8_t* const sbuf = lds + 2 * C::BUF + ((n / C::CS) & 1u) * C::SBUF;
-                stage(ring[d], buf);
-                if (in_chunk == 0u) {
-                    stage_scales(sring, sbuf);
-                    if (s + C::CS < s_hi) load_scales(sring, s + C::CS);
-                }
-                if (s + C::D < s_hi) load(ring[d], s + C::D);
-                /* a buffer is written again two steps (chunks) later: its readers passed the barrier in between */
-                lds_barrier();
-                multiply(buf, sbuf, in_chunk * C::GS);
-            }
+    load_scales(sring, s_lo);
+    load(ring, s_lo);
+    for (uint32_t s = s_lo; s < s_hi; s++) { /* (slices are not empty) */
+        const uint32_t n = s - s_lo;
+        uint8_t* const buf = lds + (n & 1u) * C::BUF;
+        uint8_t* const sbuf = lds + 2 * C::BUF + ((n / C::CS) & 1u) * C::SBUF;
+        if ((s + 1u) * KS > K) cut(ring, s);
+        stage(ring, buf);
+        if (n % C::CS == 0u) {
+            stage_scales(sring, sbuf);
+            if (s + C::CS < s_hi) load_scales(sring, s + C::CS);
         }
+        load(ring, s + 1u);
+        /* a buffer is written again two steps (chunks) later: its readers passed the barrier in between */
+        lds_barrier();
+        multiply(buf, sbuf, (n % C::CS) * C::GS);
     }
 
     /* ---- results: lane holds channel c of each 16, rows 4 q + i ---- */
@@ -389,12 +417,9 @@ template <class C>
 __global__ __launch_bounds__(C::THREADS, 2) void k_w4_tile(GroupW4 g, W4Tiles tl) {
     extern __shared__ __attribute__((aligned(16))) uint8_t w4_lds[];
     const uint32_t n0 = blockIdx.x * C::TN;
-    if (!g.meta) {
-        w4_tile<C>(g, tl, w4_lds, 0u, 0u, g.M, blockIdx.y * C::TM, n0, blockIdx.z);
-        return;
-    }
-    uint32_t e = blockIdx.y, rb = 0u, rows = 0xFFFFFFFFu;
-    if (tl.row_tiles) { /* which expert's which tile: the row tiles counted off in expert order */
+    uint32_t e = g.meta ? blockIdx.y : 0u, rb = g.meta ? 0u : blockIdx.y * C::TM, cnt = g.M, r0 = 0u;
+    const bool every = g.meta && !tl.row_tiles; /* all row tiles of one expert */
+    if (g.meta && tl.row_tiles) { /* which expert's which tile: the row tiles counted off in expert order */
         uint32_t want = blockIdx.y;
         const uint32_t lane = threadIdx.x & 63u;
         bool found = false;
@@ -411,7 +436,6 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_w4_tile(GroupW4 g, W4Tiles tl
                 const int at = __ffsll(m) - 1;
                 e = e0 + (uint32_t)at;
                 rb = (want - (uint32_t)__shfl((int)(inc - n), at, 64)) * C::TM;
-                rows = C::TM;
                 found = true;
                 break;
             }
@@ -420,20 +444,19 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_w4_tile(GroupW4 g, W4Tiles tl
         if (!found) return; /* (every wave of the workgroup counts the same) */
         e = (uint32_t)__builtin_amdgcn_readfirstlane((int)e), rb = (uint32_t)__builtin_amdgcn_readfirstlane((int)rb);
     }
-    const uint32_t cnt = (uint32_t)g.meta[g.E + e], r0 = (uint32_t)g.meta[e];
-    if (rb >= cnt) return;
-    for (int st = 0; st < C::NS; st++) {
-        const size_t at = (size_t)e * 3u + g.sel[st];
-        if (!g.wtab[at] || !g.stab[at] || (C::ASYM && !g.ztab[at])) return; /* not resident */
-    }
-    if (rows == 0xFFFFFFFFu) {
-        for (; rb < cnt; rb += C::TM) {
-            w4_tile<C>(g, tl, w4_lds, e, r0, cnt, rb, n0, 0u);
-            lds_barrier(); /* the next tile's first step may write the buffer that a slower wave still reads */
+    if (g.meta) {
+        cnt = (uint32_t)g.meta[g.E + e], r0 = (uint32_t)g.meta[e];
+        for (int st = 0; st < C::NS; st++) {
+            const size_t at = (size_t)e * 3u + g.sel[st];
+            if (!g.wtab[at] || !g.stab[at] || (C::ASYM && !g.ztab[at])) return; /* not resident */
         }
-    } else {
-        w4_tile<C>(g, tl, w4_lds, e, r0, cnt, rb, n0, 0u);
     }
+    if (rb >= cnt) return;
+    do {
+        w4_tile<C>(g, tl, w4_lds, e, r0, cnt, rb, n0, blockIdx.z);
+        lds_barrier(); /* the next tile's first step may write the buffer that a slower wave still reads */
+        rb += C::TM;
+    } while (every && rb < cnt);
 }
 
 template <class C>

@@ -5,7 +5,7 @@
 #include "w4_tile.h"
 
 template <int WT, int NS, int G, bool ASYM>
-using Cfg = W4Cfg<WT, 4, 4, NS == 2 ? 2 : 4, NS, 128, 1, 512, G, ASYM>;
+using Cfg = W4Cfg<WT, 4, 4, NS == 2 ? 2 : 4, NS, 128, 512, G, ASYM>;
 
 uint32_t w4_tiled_channels(bool glu, uint32_t) { return glu ? 128u : 256u; }
 uint32_t w4_tiled_kstep() { return 128u; }
