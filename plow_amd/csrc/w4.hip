@@ -230,6 +230,53 @@ __global__ __launch_bounds__(256) void k_w4_join(GroupW4 g, const float* __restr
     }
 }
 
+/* How a matrix-unit call is cut: rows and channels of a tile, slices of K */
+struct W4Plan {
+    uint32_t tm, tn, nt, steps, slices, steps_per;
+    bool few, wide;
+    uint64_t ns;
+};
+static W4Plan w4_shape(const GroupW4& g, bool glu, uint32_t tm, uint32_t row_tiles, uint32_t n_cu) {
+    W4Plan p = {};
+    p.tm = tm, p.few = tm <= 32u;
+    /* 32 channels per wave while that leaves every CU two workgroups: x is staged for twice the channels. 16 x 120001
+     * x 4096 G = 64 takes 67 us so and 71 us with 16; 16 x 7168 x 7168, with too few tiles for it, 17 and 15. */
+    const uint32_t tw = w4_rows_channels(glu, true);
+    p.wide = (uint64_t)((g.N + tw - 1u) / tw) * row_tiles >= 2u * n_cu;
+    p.tn = p.few ? w4_rows_channels(glu, p.wide) : w4_tiled_channels(glu);
+    const uint32_t ks = p.few ? w4_rows_kstep() : w4_tiled_kstep();
+    p.nt = (g.N + p.tn - 1u) / p.tn, p.steps = p.steps_per = (g.K + ks - 1u) / ks, p.slices = 1u;
+    return p;
+}
+/* The time a dense call takes, counted: workgroups run in rounds of what the chip holds; one takes its steps and about
+ * two more to start and end; slices of K cost their sums' way to memory and back and a second launch. A step of a
+ * full chip was measured at 1.35 us (16 rows), 1.75 (32), 2.5 and 3.3 (the same with 32 weight rows a wave; a sixth
+ * less up to two thirds full), 2.8 (64 rows; 2.2 where a CU holds one workgroup) and 2.5 (128 rows); the join at
+ * 4 us and 1 us per 2.5 MB. Picks the slices that take the least; against none they have to win by a fifteenth, since
+ * a call that streams weights at the memory's rate gains nothing from fuller rounds (16 x 120001 x 4096: 67 us, 73 in
+ * two slices). 7168 x 7168 G = 128 without slices / with: 16 rows 28 / 15 us, 64 rows 108 / 28, 128 rows 137 / 35, 512
+ * rows 138 / 82; with slices up to two workgroups a CU whatever fits / by this count: 33 rows 30 / 25, 96 rows 46 / 33 (16 rows lose:
+ * 14.7 / 15.9). */
+static W4Plan w4_dense_plan(const GroupW4& g, bool glu, uint32_t tm, uint32_t n_cu) {
+    const uint32_t gy = (g.M + tm - 1u) / tm;
+    W4Plan p = w4_shape(g, glu, tm, gy, n_cu);
+    p.ns = ~0ull;
+    if (gy > 65535u) return p; /* (the grid's limit; 128 rows always fit) */
+    const uint32_t per_cu = (uint32_t)(p.few ? w4_rows_per_cu(g, glu, p.wide, tm) : w4_tiled_per_cu(g, glu, tm));
+    const bool two = glu || p.wide;
+    const uint64_t step = tm == 16u ? (two ? 2500u : 1350u) : tm == 32u ? (two ? 3300u : 1750u) : tm == 64u && per_cu > 1u ? 2800u : tm == 64u ? 2200u : 2500u;
+    const uint64_t plane = (uint64_t)g.M * g.N * (glu ? 2u : 1u) * 4u, tiles = (uint64_t)p.nt * gy, cap = (uint64_t)n_cu * per_cu;
+    const uint32_t steps = p.steps;
+    for (uint32_t s = 1u; s == 1u || (s <= steps / 2u && tiles * (s - 1u) < 2u * cap && g.ws && plane * s <= g.ws_bytes); s++) {
+        const uint32_t per = (steps + s - 1u) / s, n = (steps + per - 1u) / per;
+        const uint64_t one = p.few && tiles * n * 3u <= cap * 2u ? step * 5u / 6u : step;
+        uint64_t ns = (tiles * n + cap - 1u) / cap * (per + 2u) * one;
+        if (n > 1u) ns = (ns + 4000u + plane * n / 2500u) * 15u / 14u;
+        if (ns < p.ns) p.ns = ns, p.slices = n, p.steps_per = per;
+    }
+    return p;
+}
+
 int launch_w4(const GroupW4& g, bool glu, hipStream_t st) {
     if (!g.N || !g.K || !g.E || !g.G || g.K % g.G) return PLOW_MOE_EINVAL;
     const uint32_t n_cu = plow_moe_n_cu();
@@ -248,43 +295,33 @@ int launch_w4(const GroupW4& g, bool glu, hipStream_t st) {
         k_w4_tiny<<<dim3((g.N + 63u) / 64u, g.E, z), 64, 0, st>>>(g, glu ? 1u : 0u);
         return 0;
     }
-    /* rows of a tile: the fewest that cover the rows at hand (routed experts: the rows of a hit expert on average) */
-    const uint32_t hit = g.slots < g.E ? g.slots : g.E;
-    const uint32_t rows = !g.meta ? g.M : g.slots ? (g.slots + hit - 1u) / hit : 1u;
-    const uint32_t tm = rows <= 16u ? 16u : rows <= 32u ? 32u : rows <= 64u ? 64u : 128u;
-    const bool few = tm <= 32u;
-    /* 32 channels per wave while that leaves every CU two workgroups */
-    const uint64_t wide_tiles = (uint64_t)((g.N + w4_rows_channels(glu, true) - 1u) / w4_rows_channels(glu, true)) * (g.meta ? hit : (g.M + tm - 1u) / tm);
-    const bool wide = wide_tiles >= 2u * n_cu;
-    const uint32_t tn = few ? w4_rows_channels(glu, wide) : w4_tiled_channels(glu, tm), ks = few ? w4_rows_kstep() : w4_tiled_kstep();
-    const uint32_t nt = (g.N + tn - 1u) / tn, steps = (g.K + ks - 1u) / ks;
     W4Tiles tl = {};
-    uint64_t gy = 1u;
+    W4Plan p;
+    uint64_t gy;
     if (!g.meta) {
-        gy = ((uint64_t)g.M + tm - 1u) / tm;
-        /* few tiles: K split over workgroups until every CU has two, two steps each at least */
-        const uint64_t tiles = nt * gy, want = 2u * n_cu;
-        if (g.ws && tiles < n_cu && steps >= 4u) {
-            uint32_t slices = (uint32_t)((want + tiles - 1u) / tiles);
-            if (slices > steps / 2u) slices = steps / 2u;
-            const uint64_t plane = (uint64_t)g.M * g.N * (glu ? 2u : 1u) * 4u;
-            if (plane * slices > g.ws_bytes) slices = (uint32_t)(g.ws_bytes / plane);
-            if (slices >= 2u) {
-                tl.steps_per = (steps + slices - 1u) / slices;
-                tl.slices = (steps + tl.steps_per - 1u) / tl.steps_per;
-                tl.part = (float*)g.ws;
-            }
+        /* dense: the rows of a tile that take the least time by the count above (128 rows of 2048 x 2816, whose weights
+         * stay in the cache: 16 rows a tile 13.6 us, 128 rows 16.2; of 7168 x 7168 58.7 and 34.7) */
+        p = w4_dense_plan(g, glu, 16u, n_cu);
+        for (uint32_t tm = 32u; tm <= 128u && tm / 2u < g.M; tm *= 2u) {
+            const W4Plan o = w4_dense_plan(g, glu, tm, n_cu);
+            if (o.ns < p.ns) p = o;
         }
-    } else if (few) {
-        gy = g.E;
+        gy = ((uint64_t)g.M + p.tm - 1u) / p.tm;
+        if (p.slices > 1u) tl.slices = p.slices, tl.steps_per = p.steps_per, tl.part = (float*)g.ws;
     } else {
-        gy = (uint64_t)g.slots / tm + hit;
-        if (gy <= 65535u) tl.row_tiles = (uint32_t)gy;
-        else gy = g.E;
+        /* routed experts: by the rows of a hit expert on average. Some get more, and a second tile reads the weights
+         * again, so that 64 rows pay from 24 on: 4096 x 1536 over 128 experts take 475 us (32 rows a tile) and 490
+         * (64) at 24 rows on average, 626 and 508 at 32, 416 and 475 at 16. Tiles of 128 rows lose by what the last
+         * one leaves empty: 2048 x 1408 over 64 experts 568 us for 554 at 240 rows, 1550 for 1493 at 768. */
+        const uint32_t hit = g.slots < g.E ? g.slots : g.E;
+        const uint32_t rows = g.slots ? (g.slots + hit - 1u) / hit : 1u;
+        p = w4_shape(g, glu, rows <= 16u ? 16u : rows <= 24u ? 32u : 64u, hit, n_cu);
+        gy = g.E;
+        if (!p.few && (uint64_t)g.slots / p.tm + hit <= 65535u) gy = tl.row_tiles = g.slots / p.tm + hit;
     }
     if (gy > 65535u) return PLOW_MOE_EINVAL;
-    const dim3 grid(nt, (uint32_t)gy, tl.slices ? tl.slices : 1u);
-    const int rc = few ? w4_rows_launch(g, tl, glu, wide, tm, grid, st) : w4_tiled_launch(g, tl, glu, tm, grid, st);
+    const dim3 grid(p.nt, (uint32_t)gy, tl.slices ? tl.slices : 1u);
+    const int rc = p.few ? w4_rows_launch(g, tl, glu, p.wide, p.tm, grid, st) : w4_tiled_launch(g, tl, glu, p.tm, grid, st);
     if (rc || !tl.slices) return rc;
     const uint64_t blocks = ((uint64_t)g.M * g.N + 255u) / 256u;
     k_w4_join<<<(uint32_t)(blocks < 4096u ? blocks : 4096u), 256, 0, st>>>(g, tl.part, tl.slices, glu ? 1u : 0u);

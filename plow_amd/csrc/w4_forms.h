@@ -7,15 +7,16 @@
 /* the kernels for a few rows read scales in runs of 64: a tensor holds one at least */
 #define W4_TINY_GROUPS 64u
 struct W4Tiles;
-/* rows of one workgroup's tile */
-enum W4Form { W4_ROWS16 = 16, W4_ROWS32 = 32, W4_ROWS64 = 64, W4_ROWS128 = 128 };
 
 uint32_t w4_rows_channels(bool glu, bool wide); /* channels of a tile; wide: 32 per wave */
 uint32_t w4_rows_kstep();
-uint32_t w4_tiled_channels(bool glu, uint32_t rows);
+uint32_t w4_tiled_channels(bool glu);
 uint32_t w4_tiled_kstep();
 int w4_rows_launch(const GroupW4& g, const W4Tiles& tl, bool glu, bool wide, uint32_t rows, dim3 grid, hipStream_t st);
 int w4_tiled_launch(const GroupW4& g, const W4Tiles& tl, bool glu, uint32_t rows, dim3 grid, hipStream_t st);
+/* workgroups of that kernel that a CU holds at once */
+int w4_rows_per_cu(const GroupW4& g, bool glu, bool wide, uint32_t rows);
+int w4_tiled_per_cu(const GroupW4& g, bool glu, uint32_t rows);
 bool w4_rows_setup();
 bool w4_tiled_setup();
 #endif

@@ -327,27 +327,39 @@ __global__ __launch_bounds__(C::THREADS, C::MTW == 1 ? 3 : 1) void k_w4_rows(Gro
 uint32_t w4_rows_channels(bool glu, bool wide) { return 64u * (!glu && wide ? 2u : 1u); }
 uint32_t w4_rows_kstep() { return 256u; }
 
+/* f(configuration that serves g) */
+template <int MTW, int NS, bool GLU, class F>
+static int by_group(const GroupW4& g, F&& f) {
+    const bool z = g.ztab || g.z[0];
+    if (g.G == 32u) return z ? f(RowsCfg<MTW, NS, GLU, 32, true>()) : f(RowsCfg<MTW, NS, GLU, 32, false>());
+    if (g.G == 64u) return z ? f(RowsCfg<MTW, NS, GLU, 64, true>()) : f(RowsCfg<MTW, NS, GLU, 64, false>());
+    return z ? f(RowsCfg<MTW, NS, GLU, 128, true>()) : f(RowsCfg<MTW, NS, GLU, 128, false>());
+}
+template <class F>
+static int by_form(const GroupW4& g, bool glu, bool wide, uint32_t rows, F&& f) {
+    if (rows == 16u) return glu ? by_group<1, 2, true>(g, f) : wide ? by_group<1, 2, false>(g, f) : by_group<1, 1, false>(g, f);
+    return glu ? by_group<2, 2, true>(g, f) : wide ? by_group<2, 2, false>(g, f) : by_group<2, 1, false>(g, f);
+}
+/* workgroups of the kernel that a CU holds, asked once */
 template <class C>
-static int rows_launch(const GroupW4& g, const W4Tiles& tl, dim3 grid, hipStream_t st) {
-    k_w4_rows<C><<<grid, C::THREADS, C::LDS, st>>>(g, tl);
-    return 0;
-}
-template <int MTW, int NS, bool GLU, int G>
-static int by_zero(const GroupW4& g, const W4Tiles& tl, dim3 grid, hipStream_t st) {
-    return (g.ztab || g.z[0]) ? rows_launch<RowsCfg<MTW, NS, GLU, G, true>>(g, tl, grid, st) : rows_launch<RowsCfg<MTW, NS, GLU, G, false>>(g, tl, grid, st);
-}
-template <int MTW, int NS, bool GLU>
-static int by_group(const GroupW4& g, const W4Tiles& tl, dim3 grid, hipStream_t st) {
-    return g.G == 32u ? by_zero<MTW, NS, GLU, 32>(g, tl, grid, st) : g.G == 64u ? by_zero<MTW, NS, GLU, 64>(g, tl, grid, st) : by_zero<MTW, NS, GLU, 128>(g, tl, grid, st);
-}
+static int rows_per_cu = 1;
+
 int w4_rows_launch(const GroupW4& g, const W4Tiles& tl, bool glu, bool wide, uint32_t rows, dim3 grid, hipStream_t st) {
-    if (rows == 16u) return glu ? by_group<1, 2, true>(g, tl, grid, st) : wide ? by_group<1, 2, false>(g, tl, grid, st) : by_group<1, 1, false>(g, tl, grid, st);
-    return glu ? by_group<2, 2, true>(g, tl, grid, st) : wide ? by_group<2, 2, false>(g, tl, grid, st) : by_group<2, 1, false>(g, tl, grid, st);
+    return by_form(g, glu, wide, rows, [&](auto c) {
+        using C = decltype(c);
+        k_w4_rows<C><<<grid, C::THREADS, C::LDS, st>>>(g, tl);
+        return 0;
+    });
+}
+int w4_rows_per_cu(const GroupW4& g, bool glu, bool wide, uint32_t rows) {
+    return by_form(g, glu, wide, rows, [](auto c) { return rows_per_cu<decltype(c)>; });
 }
 
 template <class C>
 static bool setup1() {
-    return hipFuncSetAttribute((const void*)k_w4_rows<C>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS) == hipSuccess;
+    const void* const k = (const void*)k_w4_rows<C>;
+    return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS) == hipSuccess &&
+           hipOccupancyMaxActiveBlocksPerMultiprocessor(&rows_per_cu<C>, k, C::THREADS, C::LDS) == hipSuccess;
 }
 template <int MTW, int NS, bool GLU>
 static bool setup2() {

@@ -459,13 +459,14 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_w4_tile(GroupW4 g, W4Tiles tl
     } while (every && rb < cnt);
 }
 
+/* workgroups of the kernel that a CU holds, asked once */
 template <class C>
-static int w4_launch(const GroupW4& g, const W4Tiles& tl, dim3 grid, hipStream_t st) {
-    k_w4_tile<C><<<grid, C::THREADS, C::LDS, st>>>(g, tl);
-    return 0;
-}
+static int w4_per_cu = 1;
+
 template <class C>
 static bool w4_setup() {
-    return hipFuncSetAttribute((const void*)k_w4_tile<C>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS) == hipSuccess;
+    const void* const k = (const void*)k_w4_tile<C>;
+    return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS) == hipSuccess &&
+           hipOccupancyMaxActiveBlocksPerMultiprocessor(&w4_per_cu<C>, k, C::THREADS, C::LDS) == hipSuccess;
 }
 #endif

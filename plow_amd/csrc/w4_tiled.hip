@@ -7,20 +7,31 @@
 template <int WT, int NS, int G, bool ASYM>
 using Cfg = W4Cfg<WT, 4, 4, NS == 2 ? 2 : 4, NS, 128, 512, G, ASYM>;
 
-uint32_t w4_tiled_channels(bool glu, uint32_t) { return glu ? 128u : 256u; }
+uint32_t w4_tiled_channels(bool glu) { return glu ? 128u : 256u; }
 uint32_t w4_tiled_kstep() { return 128u; }
 
-template <int WT, int NS, int G>
-static int by_zero(const GroupW4& g, const W4Tiles& tl, dim3 grid, hipStream_t st) {
-    return (g.ztab || g.z[0]) ? w4_launch<Cfg<WT, NS, G, true>>(g, tl, grid, st) : w4_launch<Cfg<WT, NS, G, false>>(g, tl, grid, st);
+/* f(Config) of the configuration that serves g */
+template <int WT, int NS, class F>
+static int by_group(const GroupW4& g, F&& f) {
+    const bool z = g.ztab || g.z[0];
+    if (g.G == 32u) return z ? f(Cfg<WT, NS, 32, true>()) : f(Cfg<WT, NS, 32, false>());
+    if (g.G == 64u) return z ? f(Cfg<WT, NS, 64, true>()) : f(Cfg<WT, NS, 64, false>());
+    return z ? f(Cfg<WT, NS, 128, true>()) : f(Cfg<WT, NS, 128, false>());
 }
-template <int WT, int NS>
-static int by_group(const GroupW4& g, const W4Tiles& tl, dim3 grid, hipStream_t st) {
-    return g.G == 32u ? by_zero<WT, NS, 32>(g, tl, grid, st) : g.G == 64u ? by_zero<WT, NS, 64>(g, tl, grid, st) : by_zero<WT, NS, 128>(g, tl, grid, st);
+template <class F>
+static int by_form(const GroupW4& g, bool glu, uint32_t rows, F&& f) {
+    if (rows == 64u) return glu ? by_group<1, 2>(g, f) : by_group<1, 1>(g, f);
+    return glu ? by_group<2, 2>(g, f) : by_group<2, 1>(g, f);
 }
 int w4_tiled_launch(const GroupW4& g, const W4Tiles& tl, bool glu, uint32_t rows, dim3 grid, hipStream_t st) {
-    if (rows == 64u) return glu ? by_group<1, 2>(g, tl, grid, st) : by_group<1, 1>(g, tl, grid, st);
-    return glu ? by_group<2, 2>(g, tl, grid, st) : by_group<2, 1>(g, tl, grid, st);
+    return by_form(g, glu, rows, [&](auto c) {
+        using C = decltype(c);
+        k_w4_tile<C><<<grid, C::THREADS, C::LDS, st>>>(g, tl);
+        return 0;
+    });
+}
+int w4_tiled_per_cu(const GroupW4& g, bool glu, uint32_t rows) {
+    return by_form(g, glu, rows, [](auto c) { return w4_per_cu<decltype(c)>; });
 }
 
 template <int WT, int NS>
