@@ -477,9 +477,11 @@ static void lp_launch(const LogprobRun& r, const LpParts& p, uint32_t grid, floa
 int launch_logprob(const LogprobRun& r, hipStream_t st) {
     const uint32_t n_cu = plow_moe_n_cu();
     if (!n_cu) return PLOW_MOE_EDEVICE;
-    /* few rows: as many workgroups per row as give every CU four, up to LP_MAX_PARTS waves of a whole tile each */
+    /* few rows: as many workgroups per row as give every CU two, up to LP_MAX_PARTS waves of a whole tile each. Rows of
+     * 120001 with a workgroup per row / so / with four per CU: 1 row f32 A = 20 34 / 13 / 13 us, 64 rows bf16 A = 5 41 /
+     * 18 / 24, 300 rows 46 / 41 / 42, 600 rows 57 / 58 / 68 (each part hands on candidates of its own). */
     const uint32_t tile = (r.f32 ? 4u : 8u) * 256u * LP_WAVES;
-    uint32_t wgs = r.T < 4u * n_cu ? (4u * n_cu + r.T - 1u) / r.T : 1u;
+    uint32_t wgs = r.T < 2u * n_cu ? (2u * n_cu + r.T - 1u) / r.T : 1u;
     const uint32_t most = r.V / tile < LP_MAX_PARTS / LP_WAVES ? r.V / tile : LP_MAX_PARTS / LP_WAVES;
     if (wgs > most) wgs = most;
     LpParts p = {};
@@ -490,7 +492,7 @@ int launch_logprob(const LogprobRun& r, hipStream_t st) {
         if (lists + parts <= r.ws_bytes) p.n = n, p.lists = (u64*)r.ws, p.part = (LpPart*)((uint8_t*)r.ws + lists);
     }
     const uint64_t grid = (uint64_t)r.T * (p.n ? p.n / LP_WAVES : 1u);
-    if (grid > 0x7FFFFFFFull) return PLOW_MOE_EINVAL;
+    if (grid >= (1ull << 24)) return PLOW_MOE_EINVAL; /* (256 threads each in 32 bits) */
     if (r.f32) {
         if (r.mask) lp_launch<true, true>(r, p, (uint32_t)grid, c2, st);
         else lp_launch<true, false>(r, p, (uint32_t)grid, c2, st);
