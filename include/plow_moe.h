@@ -126,12 +126,15 @@ enum {
      *
      * Products with 4-bit integer weights and group scales ("int4g"): W u8 [N][K / 2], low nibble = even k; S bf16 or
      * f16 [N][K / G]; Z u8 [N][K / G] with zero points 0..15, or absent: 8 everywhere. w[n][k] = (q - z) * s. The
-     * group field is G (32, 64 or 128) | PLOW_W4_SCALE_F16 when the scales are f16. K is a multiple of G (at most 2^24), N any.
+     * group field is G (32, 64 or 128) | PLOW_W4_SCALE_F16 when the scales are f16. K is a multiple of G, at most 2^24.
      * Products of bf16 activations with the exact integers q - z, f32 sums, scales applied in f32 per group.
      * Activations are finite: a row of x that holds an infinity or NaN gives infinities or NaN in its own row of out
-     * (an infinity's sign is not kept: the kernels multiply q + 16 and take (z + 16) x off again). x and the W tensors are 16-byte aligned, S is 2-byte aligned.
+     * (an infinity's sign is not kept: the kernels multiply q + 16 and take (z + 16) x off again, so that sums have to
+     * stay below 2^128 / 32). x and the W tensors are 16-byte aligned, S is 2-byte aligned. The order of a sum follows
+     * the call's sizes and the row's place in it, and is the same on every call.
      * GEMM_W4:     t0=out [M][N] t1=x bf16 [M][K] t2=W t3=S t4=Z?  i0=M i1=N i2=K i3=group field i4=x pitch in
-     *              elements (0 = K, a multiple of 8) i5=out pitch in elements (0 = N) i6=0 bf16 out, 1 f32 out
+     *              elements (0 = K, a multiple of 8) i5=out pitch in elements (0 = N) i6=0 bf16 out, 1 f32 out.
+     *              M is at most 65535 * 128, N at most 2^28
      * GEMM_GLU_W4: t0=out bf16 [M][N] t1=x t2=Wg t3=Sg t4=Zg? t5=Wu t6=Su t7=Zu?  i0=M i1=N i2=K i3=group field
      *              i4=x pitch i5=activation (0 - 4, immediates in fj[0], fj[1]) i6=out pitch */
     PLOW_DOP_X_GEMM_W4                     = 0x7001,
@@ -145,7 +148,8 @@ enum {
      *   t4=u32 [T][A]? t5=f32 [T][A]?: the A tokens of the largest logits, best first, equal logits by lowest id, and
      *      their log probabilities (either may be absent)
      *   t7=u32 [T][mask pitch]?: bit i % 32 of word i / 32 set = token i is allowed
-     *   i0=T i1=V i2=n i3=A (at most PLOW_LOGPROB_MAX_ALT) i4=logits pitch in elements (0 = V) i5=flags
+     *   i0=T (below 2^24) i1=V (below 2^31) i2=n i3=A (at most PLOW_LOGPROB_MAX_ALT) i4=logits pitch in elements
+     *   (0 = V) i5=flags
      *   i6=mask pitch in words (0 = ceil(V / 32))
      * A token that the mask forbids, or whose logit is -inf, has no probability: its log probability is -inf and it
      * is never an alternative (lists run out into id 0xFFFFFFFF, -inf), whatever a forbidden token's logit is. A row
@@ -175,7 +179,7 @@ enum {
      *   48 / 49  i6 = 16, i7 = group field, t5 = ztab?   (49 zeroes the rows of slots no expert serves)
      *   85       i3 = 16, i7 = arm 0, i6 = group field, t6 = ztab?
      *   86       i3 = 16, i7 = arm 0, i6 = group field, t5 = ztab?
-     * I and H are multiples of G. An expert is resident when its W and S (and Z, where ztab is bound) are non-null. */
+     * I and H are multiples of G, at most 65535 experts on 85 / 86. An expert is resident when its W and S (and Z, where ztab is bound) are non-null. */
     PLOW_MOE_ENC_INT4G = 16
 };
 
@@ -269,11 +273,14 @@ void plow_moe_destroy(PlowMoeCtx* ctx);
  * until plow_moe_destroy (graphs captured before stay valid) and returns PLOW_MOE_ENOMEM after seven
  * growths or when the device is out of memory. No counterpart in the reference, which quantizes every
  * gathered row inside its GEMM kernel (runtime/amd/op_moe.h:3948-4720).
- * The same block is the scratch of three other ops, each of which writes what it keeps there and reads it back
+ * The same block is the scratch of five other ops, each of which writes what it keeps there and reads it back
  * before it returns its last launch (ops of one context therefore belong on one stream at a time): op 85 arm 6 at
  * many rows (rows * (H + H / 32) bytes), the two-term arms 4 / 5 of ops 85 / 86 (aligned rows * I * 2 bytes: refused
- * when they do not fit) and the dense ops 20 / 8 (K-slice partial sums of a few rows, or the one-expert tables of
- * many: kept on their plain form when they do not fit). */
+ * when they do not fit), the dense ops 20 / 8 (K-slice partial sums of a few rows, or the one-expert tables of
+ * many: kept on their plain form when they do not fit), the dense int4 products (K-slice partial sums) and the log
+ * probabilities (partial results of a row split over workgroups): not split where the parts do not fit, and in
+ * plow_moe_exec_noalloc, which has no such block. Graphs captured from one context share the block too: replay them
+ * one after the other, or capture each from a context of its own. */
 #define PLOW_MOE_STAGE_DEFAULT_BYTES (32u << 20)
 int plow_moe_reserve_staging(PlowMoeCtx* ctx, size_t token_rows, size_t hidden);
 

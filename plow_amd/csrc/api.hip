@@ -297,6 +297,7 @@ static int w4_groups(PlowMoeCtx* c, const PlowDevInst* in, uint32_t field, Group
     NEED(c, (field & ~(0xFFFFu | PLOW_W4_SCALE_F16)) == 0u && (g->G == 32u || g->G == 64u || g->G == 128u),
          "op %u: group field 0x%x is not 32, 64 or 128 with an optional f16 scale bit", (unsigned)in->op, field);
     NEED(c, g->N && g->K && g->K % g->G == 0u && g->K <= (1u << 24), "op %u: N %u and K %u must be non-zero, K a multiple of the group size %u, at most 2^24", (unsigned)in->op, g->N, g->K, g->G);
+    NEED(c, g->N <= (1u << 28), "op %u: N %u above 2^28", (unsigned)in->op, g->N);
     NEED(c, g->act <= 4u, "op %u: activation %u is not served", (unsigned)in->op, g->act);
     return 0;
 }
@@ -382,7 +383,7 @@ static int run_w4_grouped(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, 
     else g.o_idx = (const uint32_t*)ten(in, T, 6), g.gate = (const float*)ten(in, T, 7);
     NEED(c, g.out && g.x && g.wtab && g.stab && g.meta && (glu ? g.a_idx != nullptr : (g.o_idx && g.gate)),
          "op %u: output, input, wtab, stab, meta and the row maps must be bound", (unsigned)in->op);
-    NEED(c, g.E != 0u, "op %u: zero geometry", (unsigned)in->op);
+    NEED(c, g.E != 0u && g.E <= 65535u, "op %u: %u experts, 1 .. 65535 are served", (unsigned)in->op, g.E);
     const int rc = w4_groups(c, in, i[6], &g);
     if (rc) return rc;
     NEED(c, aligned(g.x, 16u), "op %u: t1 must be 16-byte aligned", (unsigned)in->op);
@@ -402,7 +403,7 @@ static int run_logprob(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hip
     const size_t words = ((size_t)r.V + 31u) / 32u;
     r.mask_pitch = i[6] ? i[6] : words;
     NEED(c, r.logits, "logprob: t1 logits must be bound");
-    NEED(c, r.T && r.V && r.V <= 0x7FFFFFFFu, "logprob: T %u and V %u must be non-zero, V below 2^31", r.T, r.V);
+    NEED(c, r.T && r.V && r.T < (1u << 24) && r.V <= 0x7FFFFFFFu, "logprob: T %u and V %u must be non-zero, T below 2^24, V below 2^31", r.T, r.V);
     NEED(c, !r.n || (r.logprob && r.ids), "logprob: n = %u given tokens need t0 and t2", r.n);
     NEED(c, r.A <= PLOW_LOGPROB_MAX_ALT, "logprob: %u alternatives, at most %u are served", r.A, PLOW_LOGPROB_MAX_ALT);
     NEED(c, !r.A || r.alt_ids || r.alt_logprob, "logprob: %u alternatives need t4 or t5", r.A);

@@ -71,6 +71,9 @@ CASES = [
     ("product S misaligned", product(), INVAL, (3, 1)),
     ("product S at an odd element", product(), OK, (3, 2)),
     ("product out misaligned", product(i=(4, 64, 128, 32, 0, 0, 1)), INVAL, (0, 2)),
+    ("product N huge", product(i=(4, (1 << 28) + 1, 128, 32)), INVAL, None),
+    ("product M huge", product(i=(65535 * 128 + 1, 64, 128, 32)), INVAL, None),
+    ("product K huge", product(i=(4, 64, (1 << 24) + 128, 128)), INVAL, None),
     ("glu", glu(), OK, None),
     ("glu zero points", glu(t=(0, 1, 2, 3, 4, 5, 6, 7)), OK, None),
     ("glu one zero point", glu(t=(0, 1, 2, 3, 4, 5, 6)), INVAL, None),
@@ -100,6 +103,7 @@ CASES = [
     ("85 no row_token", grouped(G85, repl(T85, 5, None), I85), INVAL, None),
     ("85 no stab", grouped(G85, repl(T85, 3, None), I85), INVAL, None),
     ("85 no experts", grouped(G85, T85, repl(I85, 2, 0)), INVAL, None),
+    ("85 too many experts", grouped(G85, T85, repl(I85, 2, 65536)), INVAL, None),
     ("85 group", grouped(G85, T85, repl(I85, 6, 33)), INVAL, None),
     ("86", grouped(D86, T86, I86), OK, None),
     ("86 fused combine", grouped(D86, T86, repl(I86, 5, 2)), INVAL, None),
@@ -110,6 +114,7 @@ CASES = [
     ("logprob mask", logprob(t=(0, 1, 2, 3, 4, 5, 6, 7)), OK, None),
     ("logprob no logits", logprob(t=(0, None, 2, 3)), INVAL, None),
     ("logprob T 0", logprob(i=(0, 100, 1, 5)), INVAL, None),
+    ("logprob T huge", logprob(i=(1 << 24, 100, 1, 5)), INVAL, None),
     ("logprob V 0", logprob(i=(2, 0, 1, 5)), INVAL, None),
     ("logprob V huge", logprob(i=(2, 1 << 31, 1, 5)), INVAL, None),
     ("logprob tokens without ids", logprob(t=(0, 1, None, 3)), INVAL, None),
