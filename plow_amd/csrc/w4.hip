@@ -30,7 +30,12 @@ __global__ __launch_bounds__(256) void k_w4_zero_unserved(GroupW4 g) {
  * lane loads 16 bytes of each row per 1 KB, the next four rows' loads are issued before these are multiplied, two bit
  * operations and one v_dot2_f32_bf16 per two weights. A lane's 32 columns lie in one group: the dot product starts
  * from -(16 + z) * (their sum of x), which takes the 16 + z off again, and is scaled once. The four rows' sums meet in
- * a reduction of ten instructions: two cross-lane swaps leave one row per 16 lanes. */
+ * a reduction of ten instructions: two cross-lane swaps leave one row per 16 lanes.
+ *
+ * The weight stream bounds it: 120001 x 4096, G = 64, takes 46 us = 5.6 TB/s; eight of 384 experts of 7168 x 2048,
+ * G = 32, 35 us for gate and up (3.8 TB/s) and 16 us for down (4.3 TB/s), a few loads per wave each; 2048 x 2816 takes
+ * 4.3 us, little more than a launch. Four rows at a time: two leave too few loads in flight, eight do not fit the
+ * registers at K = 7168. */
 #define V_WAVES 4u
 
 template <int ITER, bool GLU, bool ASYM>
@@ -159,8 +164,13 @@ __global__ __launch_bounds__(V_WAVES* WAVE) void k_w4_vec(GroupW4 g, uint32_t ch
     }
 }
 
+/* a lane holds its share of the row: 64 registers at 8192 columns */
 #define W4_VEC_MAX_K 8192u
-/* Rows up to which the matrix-vector form is taken: a routing slot streams its expert's weights by itself */
+/* Which calls take the matrix-vector form: one dense row, or a few routing slots, each of which streams its expert's
+ * weights by itself (and needs no sort). Measured against the tiles of 16 rows: dense 120001 x 4096 46 us for 58, 2048 x
+ * 2816 6.4 for 8.8, 7168 x 7168 12.0 for 12.3 (two rows, one after the other: 86 for 60, 6.4 for 8.8, 17.8 for 12.7);
+ * 64 slots over 128 experts of 4096 x 1536 126 us for 144, over 384 of 7168 x 2048 296 for 350; 128 slots over the 128
+ * experts 227 for 194. */
 #define W4_VEC_MAX_SLOTS 64u
 
 bool w4_vec_serves(const GroupW4& g) {
@@ -184,7 +194,8 @@ static int launch_vec(const GroupW4& g, uint32_t n_cu, hipStream_t st) {
     return 0;
 }
 
-/* ---- tensors of fewer than 64 groups (W4_TINY_GROUPS): a thread per output ---------------------------------------- */
+/* ---- tensors of fewer than 64 groups (W4_TINY_GROUPS), which the tiles' runs of scales do not fit: a thread per
+ * output. At most 64 groups of weights: a launch's time whatever the form ---- */
 __global__ __launch_bounds__(64) void k_w4_tiny(GroupW4 g, uint32_t glu) {
     const uint32_t n = blockIdx.x * 64u + threadIdx.x, e = blockIdx.y;
     if (n >= g.N || (g.meta && !(w4_resident(g, e, g.sel[0]) && (!glu || w4_resident(g, e, g.sel[1]))))) return;
@@ -214,7 +225,8 @@ __global__ __launch_bounds__(64) void k_w4_tiny(GroupW4 g, uint32_t glu) {
     }
 }
 
-/* ---- K split: sum of the slices' partial results in slice order, through the activation for the GLU ---------- */
+/* ---- K split: sum of the slices' partial results in slice order, through the activation for the GLU. Bound by the
+ * partial sums' way from memory: 4 slices of 16 x 7168 take 3 us, 8 slices of 128 x 7168 (29 MB) 8.3 us ---- */
 __global__ __launch_bounds__(256) void k_w4_join(GroupW4 g, const float* __restrict__ part, uint32_t slices, uint32_t glu) {
     const size_t plane = (size_t)g.M * g.N;
     for (size_t i = (size_t)blockIdx.x * 256u + threadIdx.x; i < plane; i += (size_t)gridDim.x * 256u) {

@@ -8,7 +8,11 @@
  *   x        shared by the waves, 512 columns at a time: two barriers per chunk, none per step, so that the waves of
  *            a CU drift apart and one's arithmetic hides another's loads; rows that are not there are not staged
  * Twelve waves a CU (three workgroups) in 168 registers: with eight of them, two steps ahead, 64 tokens over 128
- * experts (4096 x 1536, G = 128, zero points) took 325 us for 288, four steps ahead 555. */
+ * experts (4096 x 1536, G = 128, zero points) took 325 us for 288, four steps ahead 555.
+ *
+ * What it reaches: those experts' gate and up 163 us for 843 MB (5.2 TB/s), their down, whose rows are short (6 steps),
+ * 117 us for 421 MB (3.6 TB/s); 16 rows of 120001 x 4096, G = 64, 67 us for 261 MB (3.9 TB/s); 16 rows of 7168 x 2048,
+ * G = 32, where four slices of K and their join are all latency, 8.5 + 3 us. */
 #include "w4_forms.h"
 #include "w4_tile.h"
 
@@ -114,7 +118,7 @@ __device__ __forceinline__ void w4_rows_tile(const GroupW4& g, const W4Tiles& tl
 
     /* ---- scales and zero points, a run of RUN groups at a time: whole lines. (Read chunk by chunk, 8 or 16 bytes of a
      * row each, they made a third of all requests: 16 rows of 120001 x 4096, G = 64, 77 us.) A run that would leave the
-     * tensor starts earlier; the tensor holds one run at least (w4_rows_serves). */
+     * tensor starts earlier; the tensor holds one run at least (W4_TINY_GROUPS). */
     const size_t all_groups = (size_t)N * KG;
     const uint32_t g_lo = s_lo * (C::KS / G); /* runs are counted from the slice's first group */
     auto channel = [&](uint32_t row) -> uint32_t { /* of weight row `row` of the wave's NS * 16 */

@@ -1,5 +1,5 @@
-/* w4_tile.h — the matrix-unit kernel of the int4 group-scale products (w4.hip), instantiated by w4_rows.hip (a few
- * rows) and w4_tiled.hip (many rows).
+/* w4_tile.h — the matrix-unit kernel of the int4 group-scale products (w4.hip) for many rows, instantiated by
+ * w4_tiled.hip, and what the kernel for a few rows (w4_rows.hip) shares with it.
  *
  * A workgroup computes TM rows x TN output channels (GLU: gate and up of TN channels) over a range of K, in steps of
  * KS columns. Rows of x are the A operand of v_mfma_f32_16x16x32_bf16 and weights the B operand, so a lane's four
@@ -20,7 +20,8 @@
  * Staging. Weights and x of the next step are on their way in registers (plain loads, whole 64- or 256-byte runs
  * per row); a step is written to one of two LDS buffers, one barrier per step that orders LDS only. Scales and zero
  * points come CC columns at a time, in runs of up to 64 bytes per row: read step by step, a few bytes of a line each,
- * they cost as many requests as the weights themselves. What lies behind K, behind the last row or the last channel is staged as zero, so that every step runs whole. */
+ * they cost as many requests as the weights themselves. Columns behind K count as zero, rows and channels that are not
+ * there repeat others, so that every step runs whole. */
 #ifndef PLOW_MOE_W4_TILE_H
 #define PLOW_MOE_W4_TILE_H
 
