@@ -279,7 +279,7 @@ static W4Plan w4_dense_plan(const GroupW4& g, bool glu, uint32_t tm, uint32_t n_
     const uint64_t step = tm == 16u ? (two ? 2500u : 1350u) : tm == 32u ? (two ? 3300u : 1750u) : tm == 64u && per_cu > 1u ? 2800u : tm == 64u ? 2200u : 2500u;
     const uint64_t plane = (uint64_t)g.M * g.N * (glu ? 2u : 1u) * 4u, tiles = (uint64_t)p.nt * gy, cap = (uint64_t)n_cu * per_cu;
     const uint32_t steps = p.steps;
-    for (uint32_t s = 1u; s == 1u || (s <= steps / 2u && tiles * (s - 1u) < 2u * cap && g.ws && plane * s <= g.ws_bytes); s++) {
+    for (uint32_t s = 1u; s == 1u || (s <= steps / 2u && s <= 128u && tiles * (s - 1u) < 2u * cap && g.ws && plane * s <= g.ws_bytes); s++) {
         const uint32_t per = (steps + s - 1u) / s, n = (steps + per - 1u) / per;
         const uint64_t one = p.few && tiles * n * 3u <= cap * 2u ? step * 5u / 6u : step;
         uint64_t ns = (tiles * n + cap - 1u) / cap * (per + 2u) * one;
