@@ -32,9 +32,9 @@ __global__ __launch_bounds__(256) void k_w4_zero_unserved(GroupW4 g) {
  * from -(16 + z) * (their sum of x), which takes the 16 + z off again, and is scaled once. The four rows' sums meet in
  * a reduction of ten instructions: two cross-lane swaps leave one row per 16 lanes.
  *
- * The weight stream bounds it: 120001 x 4096, G = 64, takes 46 us = 5.6 TB/s; eight of 384 experts of 7168 x 2048,
- * G = 32, 35 us for gate and up (3.8 TB/s) and 16 us for down (4.3 TB/s), a few loads per wave each; 2048 x 2816 takes
- * 4.3 us, little more than a launch. Four rows at a time: two leave too few loads in flight, eight do not fit the
+ * The weight stream bounds it: 120001 x 4096, G = 64, takes 45 us = 5.8 TB/s; eight of 384 experts of 7168 x 2048,
+ * G = 32, 49 us for gate, up, down and the combine = 4.1 TB/s, a walk of few rows per wave; 2048 x 2816 takes 4.3 us,
+ * little more than a launch. Four rows at a time: two leave too few loads in flight, eight do not fit the
  * registers at K = 7168. */
 #define V_WAVES 4u
 
@@ -46,16 +46,15 @@ struct VecRows { /* four weight rows' share of a lane */
 };
 
 template <int ITER, bool GLU, bool ASYM>
-__global__ __launch_bounds__(V_WAVES* WAVE) void k_w4_vec(GroupW4 g, uint32_t chunks, uint32_t per_chunk) {
+__global__ __launch_bounds__(V_WAVES* WAVE) void k_w4_vec(GroupW4 g, uint32_t chunks) {
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t unit = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * V_WAVES + (threadIdx.x >> 6)));
     const uint32_t row = unit / chunks, chunk = unit % chunks;
     const uint32_t N = g.N, K = g.K;
     constexpr uint32_t NC = GLU ? 2u : 4u; /* channels per four rows */
     if (row >= (g.tab ? g.nslot : g.M)) return;
-    const uint32_t q_lo = chunk * per_chunk, q_all = (N + NC - 1u) / NC;
-    const uint32_t q_hi = q_lo + per_chunk < q_all ? q_lo + per_chunk : q_all;
-    if (q_lo >= q_hi) return;
+    const uint32_t q_all = (N + NC - 1u) / NC; /* (at most as many chunks as that) */
+    const uint32_t q_lo = (uint32_t)((uint64_t)q_all * chunk / chunks), q_hi = (uint32_t)((uint64_t)q_all * (chunk + 1u) / chunks);
 
     const void *w[2] = {g.w[0], g.w[1]}, *s[2] = {g.s[0], g.s[1]}, *z[2] = {g.z[0], g.z[1]};
     float gate = 1.0f;
@@ -167,9 +166,9 @@ __global__ __launch_bounds__(V_WAVES* WAVE) void k_w4_vec(GroupW4 g, uint32_t ch
 /* a lane holds its share of the row: 64 registers at 8192 columns */
 #define W4_VEC_MAX_K 8192u
 /* Which calls take the matrix-vector form: one dense row, or a few routing slots, each of which streams its expert's
- * weights by itself (and needs no sort). Measured against the tiles of 16 rows: dense 120001 x 4096 46 us for 58, 2048 x
- * 2816 6.4 for 8.8, 7168 x 7168 12.0 for 12.3 (two rows, one after the other: 86 for 60, 6.4 for 8.8, 17.8 for 12.7);
- * 64 slots over 128 experts of 4096 x 1536 126 us for 144, over 384 of 7168 x 2048 296 for 350; 128 slots over the 128
+ * weights by itself (and needs no sort). Measured against the tiles of 16 rows: dense 120001 x 4096 45 us for 58, 2048 x
+ * 2816 6.4 for 8.8, 7168 x 7168 10.2 for 12.3 (two rows, one after the other: 86 for 60, 6.4 for 8.8, 17.8 for 12.7);
+ * 64 slots over 128 experts of 4096 x 1536 126 us for 144, over 384 of 7168 x 2048 289 for 350; 128 slots over the 128
  * experts 227 for 194. */
 #define W4_VEC_MAX_SLOTS 64u
 
@@ -182,15 +181,21 @@ template <int ITER, bool GLU>
 static int launch_vec(const GroupW4& g, uint32_t n_cu, hipStream_t st) {
     const uint32_t rows = g.tab ? g.nslot : g.M, NC = GLU ? 2u : 4u;
     const uint64_t quads = ((uint64_t)g.N + NC - 1u) / NC;
-    /* waves the chip holds at once, more of them where a row is short and a wave's registers few */
-    const uint64_t waves = (uint64_t)n_cu * (ITER == 1 ? 16u : 8u);
-    uint64_t per = (quads * rows + waves - 1u) / waves;
-    if (per == 0) per = 1;
-    if (per > quads) per = quads;
-    const uint64_t chunks = (quads + per - 1u) / per;
+    /* One set of waves walks it all, as many a CU as have enough in flight (4, 8 and 16 KB each, by the row's length):
+     * more of them fetch x more often and walk too short a run. 8 of the longest rows' waves instead of 4: eight of 384
+     * experts of 7168 x 2048 53 us for 50, 7168 x 7168 12.2 for 10.2; 8 and 16 of the middle ones instead of 12: 120001 x
+     * 4096 47 and 48.5 us for 45; 8 of the shortest instead of 16: 32000 x 2048 9.7 us for 8.7. */
+    const uint64_t waves = (uint64_t)n_cu * (ITER == 1 ? 16u : ITER == 2 ? 12u : 4u);
+    /* never more than that set (ten slots of 385 experts of 7168 x 2048: 62 us, 76 with a few waves too many), in shares
+     * that differ by one; where a share is one or two, in equal ones (14336 x 4096: 9.1 us, 11.1 unequal) */
+    uint64_t chunks = waves / rows;
+    if (chunks == 0) chunks = 1;
+    if (chunks > quads) chunks = quads;
+    const uint64_t most = (quads + chunks - 1u) / chunks;
+    if (most <= 2u) chunks = (quads + most - 1u) / most;
     const uint32_t grid = (uint32_t)((chunks * rows + V_WAVES - 1u) / V_WAVES);
-    if (g.z[0] || g.ztab) k_w4_vec<ITER, GLU, true><<<grid, V_WAVES * WAVE, 0, st>>>(g, (uint32_t)chunks, (uint32_t)per);
-    else k_w4_vec<ITER, GLU, false><<<grid, V_WAVES * WAVE, 0, st>>>(g, (uint32_t)chunks, (uint32_t)per);
+    if (g.z[0] || g.ztab) k_w4_vec<ITER, GLU, true><<<grid, V_WAVES * WAVE, 0, st>>>(g, (uint32_t)chunks);
+    else k_w4_vec<ITER, GLU, false><<<grid, V_WAVES * WAVE, 0, st>>>(g, (uint32_t)chunks);
     return 0;
 }
 
