@@ -347,6 +347,7 @@ static int run_w4_slots(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hi
     g.nslot = nslot, g.kx = kx, g.zero_unserved = glu ? 0u : 1u, g.slots = nslot;
     NEED(c, g.out && g.x && g.tab && g.wtab && g.stab, "op %u: t0 out, t1 in, t2 table, t3 weight table, t4 scale table must be bound", (unsigned)in->op);
     NEED(c, nslot && g.E, "op %u: no slots or no experts", (unsigned)in->op);
+    NEED(c, nslot % kx == 0u, "op %u: %u slots are not whole rows of %u", (unsigned)in->op, nslot, kx);
     const int wrc = w4_groups(c, in, i[7], &g);
     if (wrc) return wrc;
     NEED(c, aligned(g.x, 16u), "op %u: t1 must be 16-byte aligned", (unsigned)in->op);

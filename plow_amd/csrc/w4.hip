@@ -333,8 +333,8 @@ int launch_w4(const GroupW4& g, bool glu, hipStream_t st) {
         const uint32_t hit = g.slots < g.E ? g.slots : g.E;
         const uint32_t rows = g.slots ? (g.slots + hit - 1u) / hit : 1u;
         p = w4_shape(g, glu, rows <= 16u ? 16u : rows <= 24u ? 32u : 64u, hit, n_cu);
-        gy = g.E;
-        if (!p.few && (uint64_t)g.slots / p.tm + hit <= 65535u) gy = tl.row_tiles = g.slots / p.tm + hit;
+        gy = p.few ? g.E : (uint64_t)g.slots / p.tm + hit; /* (more row tiles than those there cannot be) */
+        if (!p.few && gy > 65535u) gy = 65535u;
     }
     if (gy > 65535u) return PLOW_MOE_EINVAL;
     const dim3 grid(p.nt, (uint32_t)gy, tl.slices ? tl.slices : 1u);

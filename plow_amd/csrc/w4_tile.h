@@ -33,7 +33,6 @@
 struct W4Tiles {
     uint32_t slices, steps_per;
     float* part;
-    uint32_t row_tiles; /* experts: an upper bound of the row tiles over all experts (grid.y), 0 = grid.y is the expert */
 };
 
 __device__ __forceinline__ float w4_f32(uint32_t h, uint32_t f16) {
@@ -412,52 +411,37 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
         }
 }
 
-/* grid: x = channel tiles, y = expert (its row tiles one after the other) or, with tl.row_tiles, row tile over all
- * experts, or dense row tile; z = K slice */
+/* grid: x = channel tiles, y = row tiles (routed experts: over all of them, from gridDim.y on the workgroups take
+ * another), z = K slice */
 template <class C>
 __global__ __launch_bounds__(C::THREADS, 2) void k_w4_tile(GroupW4 g, W4Tiles tl) {
     extern __shared__ __attribute__((aligned(16))) uint8_t w4_lds[];
-    const uint32_t n0 = blockIdx.x * C::TN;
-    uint32_t e = g.meta ? blockIdx.y : 0u, rb = g.meta ? 0u : blockIdx.y * C::TM, cnt = g.M, r0 = 0u;
-    const bool every = g.meta && !tl.row_tiles; /* all row tiles of one expert */
-    if (g.meta && tl.row_tiles) { /* which expert's which tile: the row tiles counted off in expert order */
-        uint32_t want = blockIdx.y;
-        const uint32_t lane = threadIdx.x & 63u;
-        bool found = false;
-        for (uint32_t e0 = 0; e0 < g.E; e0 += WAVE) {
-            const uint32_t n = e0 + lane < g.E ? ((uint32_t)g.meta[g.E + e0 + lane] + C::TM - 1u) / C::TM : 0u;
-            uint32_t inc = n;
-#pragma unroll
-            for (uint32_t o = 1; o < WAVE; o <<= 1) {
-                const uint32_t v = __shfl_up(inc, o, 64);
-                if (lane >= o) inc += v;
+    constexpr bool EXPERTS = C::TM == (int)PLOW_MPF_BM; /* meta counts tiles of that many rows */
+    const bool routed = EXPERTS && g.meta;
+    const int32_t* const tilep = g.meta + 2u * g.E;
+    const uint32_t n0 = blockIdx.x * C::TN, lane = threadIdx.x & 63u, total = routed ? (uint32_t)tilep[g.E] : gridDim.y;
+    uint32_t e = 0u, r0 = 0u, cnt = g.M;
+    for (uint32_t want = blockIdx.y; want < total; want += gridDim.y) {
+        uint32_t rb = want * C::TM;
+        if (routed) { /* the expert whose tiles reach past `want` first */
+            e = g.E;
+            for (uint32_t e0 = 0; e0 < g.E && e == g.E; e0 += WAVE) {
+                const uint32_t next = e0 + lane + 1u;
+                const unsigned long long m = __ballot((uint32_t)tilep[next < g.E ? next : g.E] > want);
+                if (m) e = e0 + (uint32_t)__ffsll(m) - 1u; /* (tilep[E] is total) */
             }
-            const unsigned long long m = __ballot(inc > want);
-            if (m) {
-                const int at = __ffsll(m) - 1;
-                e = e0 + (uint32_t)at;
-                rb = (want - (uint32_t)__shfl((int)(inc - n), at, 64)) * C::TM;
-                found = true;
-                break;
+            if (e >= g.E) return;
+            rb = (want - (uint32_t)tilep[e]) * C::TM, cnt = (uint32_t)g.meta[g.E + e], r0 = (uint32_t)g.meta[e];
+            bool here = rb < cnt;
+            for (int st = 0; st < C::NS; st++) {
+                const size_t at = (size_t)e * 3u + g.sel[st];
+                here = here && g.wtab[at] && g.stab[at] && (!C::ASYM || g.ztab[at]);
             }
-            want -= (uint32_t)__shfl((int)inc, 63, 64);
+            if (!here) continue; /* not resident */
         }
-        if (!found) return; /* (every wave of the workgroup counts the same) */
-        e = (uint32_t)__builtin_amdgcn_readfirstlane((int)e), rb = (uint32_t)__builtin_amdgcn_readfirstlane((int)rb);
-    }
-    if (g.meta) {
-        cnt = (uint32_t)g.meta[g.E + e], r0 = (uint32_t)g.meta[e];
-        for (int st = 0; st < C::NS; st++) {
-            const size_t at = (size_t)e * 3u + g.sel[st];
-            if (!g.wtab[at] || !g.stab[at] || (C::ASYM && !g.ztab[at])) return; /* not resident */
-        }
-    }
-    if (rb >= cnt) return;
-    do {
         w4_tile<C>(g, tl, w4_lds, e, r0, cnt, rb, n0, blockIdx.z);
         lds_barrier(); /* the next tile's first step may write the buffer that a slower wave still reads */
-        rb += C::TM;
-    } while (every && rb < cnt);
+    }
 }
 
 /* workgroups of the kernel that a CU holds, asked once */

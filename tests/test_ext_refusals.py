@@ -87,6 +87,8 @@ CASES = [
     ("48 no table", slots(G48, t=(0, 1, None, 3, 4)), INVAL, None),
     ("48 no scales", slots(G48, t=(0, 1, 2, 3)), INVAL, None),
     ("48 no slots", slots(G48, i=(0, 64, 128, 4, 2, 1, 16, 32)), INVAL, None),
+    ("48 part of a row", slots(G48, i=(8, 64, 128, 4, 3, 1, 16, 32)), INVAL, None),
+    ("48 one shared row", slots(G48, i=(7, 64, 128, 4, 0, 1, 16, 32)), OK, None),
     ("48 no experts", slots(G48, i=(8, 64, 128, 0, 2, 1, 16, 32)), INVAL, None),
     ("48 too many experts", slots(G48, i=(8, 64, 128, 1057, 2, 1, 16, 32)), INVAL, None),
     ("48 too many slots", slots(G48, i=((1 << 20) + 1, 64, 128, 4, 2, 1, 16, 32)), INVAL, None),

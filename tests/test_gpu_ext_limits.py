@@ -173,6 +173,36 @@ def test_one_expert_for_every_slot_and_twice_in_a_token(moe, T, E, k):
     routed(E, 384, 128, 32, eid, run)
 
 
+@pytest.mark.parametrize("stated", [150, 600, 1 << 20, 0xFFFFFFFF])
+def test_gathered_rows_whatever_count_is_stated(moe, stated):
+    """The row count that a grouped op may state chooses a form and a grid; a wrong one costs time, not rows."""
+    print(f"[case] gathered, stated {stated}", flush=True)
+    T, E, k, H, I, G = 200, 5, 3, 256, 192, 64
+    sets, tabs = experts(E, H, I, G, 3)
+    eid = torch.randint(0, E, (T, k), generator=ec.gen(1), dtype=torch.int32)
+    eid[: T // 2, 0] = 3
+    gate = torch.rand(T, k, generator=ec.gen(2)) + 0.1
+    tab = torch.stack([eid, gate.view(torch.int32)], 2).reshape(T * k, 2).contiguous().cuda()
+    x = torch.randn(T, H, generator=gen(5), device="cuda").to(torch.bfloat16)
+    R = abi.max_rows(T, k, E)
+    fu, part = torch.zeros(R, I, dtype=torch.bfloat16, device="cuda"), torch.full((T * k + 1, H), 3.0, device="cuda")
+    maps = [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (3 * E + 1, R, R, R)]
+    tensors = ec.table_of([fu, x, tab, *tabs, part, *maps])
+    for d in (abi.inst(abi.OP_MOE_ALIGN_PF, t=[7, 2, 8, 9, 10], i=[T, E, k]),
+              abi.inst(abi.OP_MOE_GROUP_GLU_PF, t=[0, 1, 3, 4, 7, 8, 5], i=[I, H, E, abi.ENC_INT4G, 0, abi.ACT_SILU, G, abi.ARM_A16], slots=stated),
+              abi.inst(abi.OP_MOE_GROUP_DOWN_PF, t=[6, 0, 3, 4, 7, 5, 9, 10], i=[H, I, E, abi.ENC_INT4G, 0, 0, G, abi.ARM_A16], slots=stated)):
+        moe.exec(d, tensors)
+    torch.cuda.synchronize()
+    assert (part[-1] == 3).all()
+    for e in range(E):
+        s = (eid.view(-1) == e).nonzero()[:, 0]
+        d = [ec.dequant64(*m[e]).T.contiguous() for m in sets]
+        xr = x[(s // k).cuda()].double()
+        # the intermediate rounds to bf16: half a step of each value, spread evenly, 0.58 of it in the mean square
+        want = ec.act64(xr @ d[0], xr @ d[1], abi.ACT_SILU) @ d[2] * gate.view(-1)[s].cuda().double()[:, None]
+        assert (part[s.cuda()].double() - want).norm() <= 0.65 * HALF_BF16 * want.norm(), e
+
+
 @pytest.mark.parametrize("T", [2, 50, 400])
 def test_experts_without_a_context(moe, T):
     fn = moe.lib.plow_moe_exec_noalloc
