@@ -297,6 +297,9 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
 
     const W4Bits bits = w4_bits();
     v4f acc[NS][C::NBW][C::MTW] = {};
+    /* Instruction by instruction over all of the wave's tiles: 16 sums grow side by side, none waits for the one before
+     * it, and x is read as it is needed. (Tile by tile, a group's instructions after one another: 2048 x 4096 x 7168 142 us
+     * for 133.) */
     constexpr int TILES = NS * C::NBW;
     auto multiply = [&](const uint8_t* buf, const uint8_t* sbuf, uint32_t g0) { /* g0: the step's first group in its chunk */
         const uint8_t* const xl = buf + (wt * C::MTW * 16u + c) * C::XROW;
@@ -306,55 +309,54 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
         const uint8_t* const zl = sbuf + C::S_BYTES + (wc * C::NBW * 16u + c) * C::ZROW + g0;
 #pragma unroll
         for (int blk = 0; blk < KS / 128; blk++) {
-            /* a lane's 32 weights of 16 channels: one group (G = 128) is read one turn ahead, several stay */
-            constexpr int RAW = G == 128 ? 2 : TILES;
-            uint32_t raw[RAW][4];
-            auto fetch = [&](int i) {
+            uint32_t raw[TILES][4]; /* a lane's 32 weights of each 16 channels */
+#pragma unroll
+            for (int i = 0; i < TILES; i++) {
                 const v4i w = *(const v4i*)(wl + ((i / C::NBW) * C::TN + wc * C::NBW * 16u + (i % C::NBW) * 16u + c) * C::WROW + blk * 64u + q * 16u);
 #pragma unroll
-                for (int k = 0; k < 4; k++) raw[i % RAW][k] = (uint32_t)w[k];
-                w4_deal<G>(raw[i % RAW]);
-            };
-#pragma unroll
-            for (int i = 0; i < (G == 128 ? 1 : TILES); i++) fetch(i);
+                for (int k = 0; k < 4; k++) raw[i][k] = (uint32_t)w[k];
+                w4_deal<G>(raw[i]);
+            }
             constexpr int RG = G / 32; /* instructions per group */
 #pragma unroll
             for (int gr = 0; gr < 128 / G; gr++) {
                 const int gi = blk * (128 / G) + gr;
-                v4f cx[C::MTW];
-                v8bf a[C::MTW][RG];
+                v4f cx[C::MTW], t[TILES][C::MTW];
 #pragma unroll
-                for (int mt = 0; mt < C::MTW; mt++) {
-                    cx[mt] = *(const v4f*)(xs + gi * C::TM + mt * 16);
+                for (int mt = 0; mt < C::MTW; mt++) cx[mt] = *(const v4f*)(xs + gi * C::TM + mt * 16);
 #pragma unroll
-                    for (int r = 0; r < RG; r++)
-                        a[mt][r] = *(const v8bf*)(xl + mt * 16 * C::XROW + (blk * 128u + w4_koff<G>(q, gr * RG + r)) * 2u);
-                }
+                for (int r = 0; r < RG; r++) {
+                    const int at = gr * RG + r;
+                    v8bf a[C::MTW];
 #pragma unroll
-                for (int st = 0; st < NS; st++)
+                    for (int mt = 0; mt < C::MTW; mt++) a[mt] = *(const v8bf*)(xl + mt * 16 * C::XROW + (blk * 128u + w4_koff<G>(q, at)) * 2u);
 #pragma unroll
-                    for (int nb = 0; nb < C::NBW; nb++) {
-                        const float s = w4_f32(*(const uint16_t*)(sl + (st * C::TN + nb * 16) * C::SROW + gi * 2), g.s_f16);
-                        const float zc = C::ASYM ? 16.0f + (float)zl[(st * C::TN + nb * 16) * C::ZROW + gi] : 0.0f;
-                        const int i = st * C::NBW + nb;
-                        if (G == 128 && i + 1 < TILES) fetch(i + 1);
-                        v8bf b[RG];
-#pragma unroll
-                        for (int r = 0; r < RG; r++) b[r] = w4_unpack(raw[i % RAW][gr * RG + r], bits);
+                    for (int i = 0; i < TILES; i++) {
+                        const v8bf b = w4_unpack(raw[i][at], bits);
+                        float zc = 0.0f;
+                        if (C::ASYM && r == 0) zc = 16.0f + (float)zl[((i / C::NBW) * C::TN + (i % C::NBW) * 16) * C::ZROW + gi];
 #pragma unroll
                         for (int mt = 0; mt < C::MTW; mt++) {
-                            v4f t = cx[mt];
-                            if (C::ASYM) {
+                            v4f from = r ? t[i][mt] : cx[mt];
+                            if (C::ASYM && r == 0) {
 #pragma unroll
-                                for (int i = 0; i < 4; i++) t[i] *= zc;
+                                for (int k = 0; k < 4; k++) from[k] *= zc;
                             }
-#pragma unroll
-                            for (int r = 0; r < RG; r++) t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mt][r], b[r], t, 0, 0, 0);
-#pragma unroll
-                            for (int i = 0; i < 4; i++) acc[st][nb][mt][i] = fmaf(t[i], s, acc[st][nb][mt][i]);
+                            t[i][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mt], b, from, 0, 0, 0);
                         }
-                        __builtin_amdgcn_sched_barrier(0); /* (more in flight at once does not fit the registers) */
                     }
+                    /* the four-wave form does not fit its registers with more reads moved up: 64 rows of 7168 x 7168 31 us
+                     * for 27.5 (128 rows run alike, with groups of 32 slower for it: 239 us for 218) */
+                    if (C::WT == 1) __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int i = 0; i < TILES; i++) {
+                    const float sc = w4_f32(*(const uint16_t*)(sl + ((i / C::NBW) * C::TN + (i % C::NBW) * 16) * C::SROW + gi * 2), g.s_f16);
+#pragma unroll
+                    for (int mt = 0; mt < C::MTW; mt++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) acc[i / C::NBW][i % C::NBW][mt][k] = fmaf(t[i][mt][k], sc, acc[i / C::NBW][i % C::NBW][mt][k]);
+                }
             }
         }
     };
