@@ -345,9 +345,10 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
                             t[i][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mt], b, from, 0, 0, 0);
                         }
                     }
-                    /* the four-wave form does not fit its registers with more reads moved up: 64 rows of 7168 x 7168 31 us
-                     * for 27.5 (128 rows run alike, with groups of 32 slower for it: 239 us for 218) */
-                    if (C::WT == 1) __builtin_amdgcn_sched_barrier(0);
+                    /* the four-wave forms do not fit their registers with more reads moved up: 64 rows of 7168 x 7168 31 us for
+                     * 27.5, a GLU of groups of 64 with zero points 850 for 819; but for the GLU of groups of 128 without: 176
+                     * for 183. (The eight-wave forms do; groups of 32 take 239 us for 218 with it.) */
+                    if (C::WT == 1 && !(NS == 2 && G == 128 && !C::ASYM)) __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
                 for (int i = 0; i < TILES; i++) {
