@@ -271,8 +271,8 @@ static W4Plan w4_shape(const GroupW4& g, bool glu, uint32_t tm, uint32_t row_til
  * less up to two thirds full), 2.8 (64 rows; 2.2 where a CU holds one workgroup) and 2.5 (128 rows); the join at
  * 4 us and 1 us per 2.5 MB. Picks the slices that take the least; against none they have to win by a fifteenth, since
  * a call that streams weights at the memory's rate gains nothing from fuller rounds (16 x 120001 x 4096: 67 us, 73 in
- * two slices). 7168 x 7168 G = 128 without slices / with: 16 rows 28 / 15 us, 64 rows 108 / 28, 128 rows 137 / 35, 512
- * rows 138 / 82; with slices up to two workgroups a CU whatever fits / by this count: 33 rows 30 / 25, 96 rows 46 / 33 (16 rows lose:
+ * two slices). 7168 x 7168 G = 128 without slices / with: 16 rows 28 / 16 us, 64 rows 108 / 28, 128 rows 137 / 34, 512
+ * rows 138 / 75; with slices up to two workgroups a CU whatever fits / by this count: 33 rows 30 / 25, 96 rows 46 / 33 (16 rows lose:
  * 14.7 / 15.9). */
 static W4Plan w4_dense_plan(const GroupW4& g, bool glu, uint32_t tm, uint32_t n_cu) {
     const uint32_t gy = (g.M + tm - 1u) / tm;
