@@ -1,4 +1,4 @@
-/* w4_forms.h — the instances of the int4 matrix-unit kernel (w4_tile.h) by name, for the dispatch in w4.hip. */
+/* w4_forms.h — the int4 matrix-unit kernels (w4_rows.hip, w4_tiled.hip) as the dispatch in w4.hip sees them. */
 #ifndef PLOW_MOE_W4_FORMS_H
 #define PLOW_MOE_W4_FORMS_H
 

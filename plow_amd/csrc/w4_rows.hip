@@ -363,7 +363,7 @@ template <class C>
 static bool setup1() {
     const void* const k = (const void*)k_w4_rows<C>;
     return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS) == hipSuccess &&
-           hipOccupancyMaxActiveBlocksPerMultiprocessor(&rows_per_cu<C>, k, C::THREADS, C::LDS) == hipSuccess;
+           hipOccupancyMaxActiveBlocksPerMultiprocessor(&rows_per_cu<C>, k, C::THREADS, C::LDS) == hipSuccess && rows_per_cu<C> > 0;
 }
 template <int MTW, int NS, bool GLU>
 static bool setup2() {

@@ -455,6 +455,6 @@ template <class C>
 static bool w4_setup() {
     const void* const k = (const void*)k_w4_tile<C>;
     return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS) == hipSuccess &&
-           hipOccupancyMaxActiveBlocksPerMultiprocessor(&w4_per_cu<C>, k, C::THREADS, C::LDS) == hipSuccess;
+           hipOccupancyMaxActiveBlocksPerMultiprocessor(&w4_per_cu<C>, k, C::THREADS, C::LDS) == hipSuccess && w4_per_cu<C> > 0;
 }
 #endif
