@@ -148,8 +148,8 @@ enum {
      *   t4=u32 [T][A]? t5=f32 [T][A]?: the A tokens of the largest logits, best first, equal logits by lowest id, and
      *      their log probabilities (either may be absent)
      *   t7=u32 [T][mask pitch]?: bit i % 32 of word i / 32 set = token i is allowed
-     *   i0=T (below 2^24) i1=V (below 2^31) i2=n i3=A (at most PLOW_LOGPROB_MAX_ALT) i4=logits pitch in elements
-     *   (0 = V) i5=flags
+     *   i0=T (below 2^24) i1=V (below 2^31) i2=n (below 2^31) i3=A (at most PLOW_LOGPROB_MAX_ALT) i4=logits pitch in
+     *   elements (0 = V) i5=flags
      *   i6=mask pitch in words (0 = ceil(V / 32))
      * A token that the mask forbids, or whose logit is -inf, has no probability: its log probability is -inf and it
      * is never an alternative (lists run out into id 0xFFFFFFFF, -inf), whatever a forbidden token's logit is. A row

@@ -406,6 +406,7 @@ static int run_logprob(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hip
     NEED(c, r.logits, "logprob: t1 logits must be bound");
     NEED(c, r.T && r.V && r.T < (1u << 24) && r.V <= 0x7FFFFFFFu, "logprob: T %u and V %u must be non-zero, T below 2^24, V below 2^31", r.T, r.V);
     NEED(c, !r.n || (r.logprob && r.ids), "logprob: n = %u given tokens need t0 and t2", r.n);
+    NEED(c, r.n <= 0x7FFFFFFFu, "logprob: %u given tokens a row, below 2^31 are served", r.n); /* (a wave counts them 64 at a time in 32 bits) */
     NEED(c, r.A <= PLOW_LOGPROB_MAX_ALT, "logprob: %u alternatives, at most %u are served", r.A, PLOW_LOGPROB_MAX_ALT);
     NEED(c, !r.A || r.alt_ids || r.alt_logprob, "logprob: %u alternatives need t4 or t5", r.A);
     NEED(c, r.n || r.A || r.entropy || r.lse, "logprob: no output is asked for");
