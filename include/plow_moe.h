@@ -127,7 +127,9 @@ enum {
      * Products with 4-bit integer weights and group scales ("int4g"): W u8 [N][K / 2], low nibble = even k; S bf16 or
      * f16 [N][K / G]; Z u8 [N][K / G] with zero points 0..15, or absent: 8 everywhere. w[n][k] = (q - z) * s. The
      * group field is G (32, 64 or 128) | PLOW_W4_SCALE_F16 when the scales are f16. K is a multiple of G, at most 2^24.
-     * Products of bf16 activations with the exact integers q - z, f32 sums, scales applied in f32 per group.
+     * Products of bf16 activations with the exact integers q - z, f32 sums, scales applied in f32 per group. The sums
+     * run over (16 + q) x and have (16 + z) x taken off again: an output is off by at most 2 K * 2^-24 times the sum of
+     * s (32 + q + z) |x|, in a group whose weights are all zero (q = z) too. Scale 0 makes such a group's share exactly 0.
      * Activations are finite: a row of x that holds an infinity or NaN gives infinities or NaN in its own row of out
      * (an infinity's sign is not kept: the kernels multiply q + 16 and take (z + 16) x off again, so that sums have to
      * stay below 2^128 / 32). x and the W tensors are 16-byte aligned, S is 2-byte aligned. The order of a sum follows

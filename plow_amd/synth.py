@@ -83,19 +83,25 @@ def quant_mxfp4(w: torch.Tensor):
 def quant_int4_group(w: torch.Tensor, group: int, zero_points: bool = False, scale_f16: bool = False):
     """w [N, K] -> (packed u8 [N, K/2] low nibble = even k, scales bf16 | f16 [N, K/group], zero points u8 or None).
     Symmetric: scale amax / 7, codes round(w / scale) + 8 in 1..15; with zero points: scale (max - min) / 15 over a
-    range that holds 0, code and zero point in 0..15. Codes are taken with the scale as stored."""
+    range that holds 0, code and zero point in 0..15. Codes are taken with the scale as stored; a group of zeros has
+    scale 0, so that its share of a product is exactly 0. A range that no scale of the type holds is refused."""
     N, K = w.shape
     blk = w.float().view(N, K // group, group)
     dt = torch.float16 if scale_f16 else torch.bfloat16
+    fi = torch.finfo(dt)
     if zero_points:
         lo, hi = blk.amin(2).clamp(max=0.0), blk.amax(2).clamp(min=0.0)
-        scale = torch.where(hi > lo, (hi - lo) / 15.0, torch.ones_like(hi)).to(dt)
-        zero = (-lo / scale.float()).round().clamp(0, 15)
+        scale = (hi - lo) / 15.0
     else:
-        amax = blk.abs().amax(2)
-        scale = torch.where(amax > 0, amax / 7.0, torch.ones_like(amax)).to(dt)
-        zero = torch.full_like(amax, 8.0)
-    q = ((blk / scale.float().unsqueeze(2)).round() + zero.unsqueeze(2)).clamp(0, 15).to(torch.uint8).view(N, K)
+        scale = blk.abs().amax(2) / 7.0
+    if not bool((scale <= fi.max).all()):      # (NaN too)
+        raise ValueError(f"quant_int4_group: a group's range does not fit a scale of {dt}")
+    # a subnormal scale rounds up, so that the largest weight keeps a code
+    sub = fi.smallest_normal * fi.eps
+    scale = torch.where(scale < fi.smallest_normal, (scale / sub).ceil() * sub, scale).to(dt)
+    div = torch.where(scale > 0, scale.float(), torch.ones_like(scale, dtype=torch.float32))
+    zero = (-lo / div).round().clamp(0, 15) if zero_points else torch.full_like(div, 8.0)
+    q = ((blk / div.unsqueeze(2)).round() + zero.unsqueeze(2)).clamp(0, 15).to(torch.uint8).view(N, K)
     packed = (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous()
     return packed, scale.contiguous(), zero.to(torch.uint8).contiguous() if zero_points else None
 
