@@ -141,8 +141,8 @@ enum {
      *              i4=x pitch i5=activation (0 - 4, immediates in fj[0], fj[1]) i6=out pitch */
     PLOW_DOP_X_GEMM_W4                     = 0x7001,
     PLOW_DOP_X_GEMM_GLU_W4                 = 0x7002,
-    /* Log probabilities of tokens from rows of logits, with c = fj[0] (0 reads as 1; positive, at most 1e30) multiplying
-     * every logit (1 / temperature):
+    /* Log probabilities of tokens from rows of logits, with c = fj[0] (0 reads as 1; 1e-30 .. 1e30) multiplying every
+     * logit (1 / temperature):
      *   t1=logits [T][pitch] (bf16, or f32 with PLOW_LOGPROB_F32 in i5)
      *   t0=f32 [T][n]: log probability of token t2[r][j] (u32 [T][n]). Token 0xFFFFFFFF asks for nothing (0 is
      *      written), any other id >= V gives NaN
@@ -154,7 +154,8 @@ enum {
      *   elements (0 = V) i5=flags
      *   i6=mask pitch in words (0 = ceil(V / 32))
      * A token that the mask forbids, or whose logit is -inf, has no probability: its log probability is -inf and it
-     * is never an alternative (lists run out into id 0xFFFFFFFF, -inf), whatever a forbidden token's logit is. A row
+     * is never an alternative (lists run out into id 0xFFFFFFFF, -inf), whatever a forbidden token's logit is. Any
+     * other log probability is finite unless c (logit - largest) itself is past the largest f32. A row
      * with no token left: log of the sum -inf, entropy 0. An allowed NaN or +inf makes the row's f32 outputs NaN
      * (both rank ahead of every number, NaN first). Logits are aligned to their element; f32 sums throughout. */
     PLOW_DOP_X_LOGPROB                     = 0x7010

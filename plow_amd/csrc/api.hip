@@ -413,7 +413,8 @@ static int run_logprob(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hip
     NEED(c, r.pitch >= r.V, "logprob: logits pitch %zu below V %u", r.pitch, r.V);
     NEED(c, r.mask_pitch >= words, "logprob: mask pitch %zu below the %zu words of V %u", r.mask_pitch, words, r.V);
     NEED(c, (i[5] & ~PLOW_LOGPROB_F32) == 0u && i[7] == 0u, "logprob: unknown flags 0x%x (i5) or 0x%x (i7)", i[5], i[7]);
-    NEED(c, r.scale > 0.0f && r.scale <= 1e30f, "logprob: scale (f0) must be positive, at most 1e30");
+    /* (from there on e^(c (x - m)) is 0 for every difference past the largest f32) */
+    NEED(c, r.scale >= 1e-30f && r.scale <= 1e30f, "logprob: scale (f0) must lie in 1e-30 .. 1e30");
     NEED(c, aligned(r.logits, r.f32 ? 4u : 2u) && aligned(r.logprob, 4u) && aligned(r.ids, 4u) && aligned(r.entropy, 4u) && aligned(r.lse, 4u) &&
                 aligned(r.alt_ids, 4u) && aligned(r.alt_logprob, 4u) && aligned(r.mask, 4u), "logprob: every tensor must be aligned to its element");
     if (!launch) return 0;

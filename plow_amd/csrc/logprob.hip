@@ -322,7 +322,8 @@ __device__ __forceinline__ void lp_write(const LogprobRun& r, size_t row, const 
     const float NINF = -__builtin_inff(), LN2 = 0.69314718055994531f;
     const float base = s.m == NINF ? 0.0f : s.m, logz = logf(s.z);
     const bool bad = s.z != s.z;
-    auto logp = [&](float x) { return bad ? s.z : x == NINF ? NINF : (x - base) * r.scale - logz; };
+    /* halves: the difference of two finite logits may be past the largest f32 where c times it is not */
+    auto logp = [&](float x) { return bad ? s.z : x == NINF ? NINF : (0.5f * x - 0.5f * base) * (2.0f * r.scale) - logz; };
     if (lane == 0u) {
         if (r.entropy) r.entropy[row] = s.z == 0.0f ? 0.0f : logz - s.t * LN2 / s.z;
         if (r.lse) r.lse[row] = bad ? s.z : base * r.scale + logz;

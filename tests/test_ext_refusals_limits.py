@@ -13,6 +13,12 @@ CASES = [
     ("given tokens at the limit", logprob(i=(2, 100, 0x7FFFFFFF, 5)), OK),
     ("given tokens past the limit", logprob(i=(2, 100, 0x80000000, 5)), INVAL),
     ("given tokens that wrap", logprob(i=(2, 100, 0xFFFFFFFF, 5)), INVAL),
+    # a factor so small that logits further apart than the largest f32 would count
+    ("smallest scale", logprob(f=(1e-30,)), OK),
+    ("largest scale", logprob(f=(1e30,)), OK),
+    ("scale below", logprob(f=(9e-31,)), INVAL),
+    ("scale subnormal", logprob(f=(1e-42,)), INVAL),
+    ("scale above", logprob(f=(1.1e30,)), INVAL),
 ]
 
 

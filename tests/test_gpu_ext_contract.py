@@ -1,0 +1,52 @@
+"""What the int4 and log-probability ops promise beyond their formulas: finite log probabilities wherever the value is
+representable, the same bits on every call whatever staging the context holds, a kernel form that follows the call's
+rows."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import ext_cases as ec
+from plow_amd import abi
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def moe():
+    from plow_amd.lib import Moe
+    m = Moe(0)
+    yield m
+    m.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [50, 20000])
+@pytest.mark.parametrize("scale", [0.25, 0.49, 1e-30])
+def test_logits_further_apart_than_a_type_reaches(moe, V, dtype, scale):
+    """Largest minus smallest logit is past the largest f32, the log probability c (x - m) - ln Z is not."""
+    print(f"[case] far apart V={V} {dtype} c={scale}", flush=True)
+    T, A, top = 3, 7, torch.finfo(dtype).max
+    x = torch.randn(T, V, generator=ec.gen(V))
+    x[:, 5] = top
+    x[0, 9] = -top
+    x[1, V - 1] = -top * 0.99
+    x[2, 6:] = -top
+    x[2, 20] = 0.0
+    x = x.to(dtype)
+    ids = torch.tensor([[9, 5], [V - 1, 0], [6, 20]], dtype=torch.int32)
+    c = float(np.float32(scale))
+    want = ec.logprob64(x, V, ids, A, c)
+    lp, ent, lse = torch.zeros(T, 2, device="cuda"), torch.zeros(T, device="cuda"), torch.zeros(T, device="cuda")
+    aid, alp = torch.zeros(T, A, dtype=torch.int32, device="cuda"), torch.zeros(T, A, device="cuda")
+    moe.exec(abi.inst(abi.OP_X_LOGPROB, t=[0, 1, 2, 3, 4, 5, 6], i=[T, V, 2, A, 0, abi.LOGPROB_F32 if dtype == torch.float32 else 0], f=[scale]),
+             ec.table_of([lp, x.cuda(), ids.cuda(), ent, aid, alp, lse]))
+    torch.cuda.synchronize()
+    assert torch.equal(aid.cpu(), want["alt_ids"])
+    # x - m, c times it and ln Z taken off: a rounding each; every other token's e^d is 0, so that ln Z and the entropy
+    # are 0, and c m of the log of the sum rounds once
+    for got, k in ((lp, "logprob"), (ent, "entropy"), (lse, "lse"), (alp, "alt_logprob")):
+        got = got.cpu().double()
+        assert torch.isfinite(got).all(), (k, got)
+        assert ((got - want[k]).abs() <= 3 * ec.EPS_F32 * want[k].abs()).all(), (k, got, want[k])
