@@ -1239,7 +1239,7 @@ static int check_segment(PlowMoeCtx* c, const PlowDevInst* insts, uint32_t n) {
     } else {
         NEED(c, g.i[1] == d.i[2] && g.i[2] == d.i[1] && g.i[3] == d.i[3], "segment: GLU (I,H,E) and DOWN (H,I,E) disagree");
         NEED(c, g.t[0] == d.t[1] && g.t[2] == d.t[2] && g.t[3] == d.t[3], "segment: fu / table / weight-table handles differ");
-        if (g.op == PLOW_DOP_MOE_GROUP_GLU_FP8_BLK && g.i[6] == PLOW_MOE_ENC_INT4G)
+        if (g.op == PLOW_DOP_MOE_GROUP_GLU_FP8_BLK && (g.i[6] == PLOW_MOE_ENC_INT4G || d.i[6] == PLOW_MOE_ENC_INT4G))
             NEED(c, d.i[6] == g.i[6] && g.t[5] == d.t[5], "segment: weight encodings or ztab handles differ");
     }
     return 0;

@@ -27,3 +27,15 @@ def test_limits_on_the_host(host_lib, host_ctx, case):  # noqa: F811
     name, inst, code = case
     got = host_lib.plow_moe_check(host_ctx, C.byref(inst), table(1 << 32, None))
     assert got == code, (name, got, host_lib.plow_moe_last_error(host_ctx).decode())
+
+
+@pytest.mark.parametrize("glu_enc,down_enc", [(2, 16), (1, 16), (0, 16), (16, 2), (16, 1), (16, 0)])
+def test_segments_of_mixed_encodings_on_the_host(host_lib, host_ctx, glu_enc, down_enc):  # noqa: F811
+    """GLU and DOWN of one weight table are both int4 or neither: an int4 DOWN behind another GLU is refused like the
+    reverse. (An op that no library serves ends the run, so that a pair let through is not launched.)"""
+    def enc(at):
+        return 32 if at == 16 else 0
+    run = [slots(G48, i=(8, 128, 128, 4, 2, 1, glu_enc, enc(glu_enc))),
+           slots(D49, t=(6, 0, 2, 3, 4), i=(8, 128, 128, 4, 0, 0, down_enc, enc(down_enc))), abi.inst(0x7FFF, t=[], i=[])]
+    assert host_lib.plow_moe_dec(host_ctx, abi.inst_array(run), 3, table(1 << 32, None), 4, None) == INVAL
+    assert b"segment" in host_lib.plow_moe_last_error(host_ctx)
