@@ -133,7 +133,8 @@ enum {
      * Activations are finite: a row of x that holds an infinity or NaN gives infinities or NaN in its own row of out
      * (an infinity's sign is not kept: the kernels multiply q + 16 and take (z + 16) x off again, so that sums have to
      * stay below 2^128 / 32). x and the W tensors are 16-byte aligned, S is 2-byte aligned. The order of a sum follows
-     * the call's sizes and the row's place in it, and is the same on every call.
+     * the call's sizes and the row's place in it: the bits are the same on every call of every context, whatever staging
+     * it has reserved. plow_moe_exec_noalloc, which never splits K, may order a dense call's sums differently.
      * GEMM_W4:     t0=out [M][N] t1=x bf16 [M][K] t2=W t3=S t4=Z?  i0=M i1=N i2=K i3=group field i4=x pitch in
      *              elements (0 = K, a multiple of 8) i5=out pitch in elements (0 = N) i6=0 bf16 out, 1 f32 out.
      *              M is at most 65535 * 128, N at most 2^28
@@ -280,9 +281,10 @@ void plow_moe_destroy(PlowMoeCtx* ctx);
  * before it returns its last launch (ops of one context therefore belong on one stream at a time): op 85 arm 6 at
  * many rows (rows * (H + H / 32) bytes), the two-term arms 4 / 5 of ops 85 / 86 (aligned rows * I * 2 bytes: refused
  * when they do not fit), the dense ops 20 / 8 (K-slice partial sums of a few rows, or the one-expert tables of
- * many: kept on their plain form when they do not fit), the dense int4 products (K-slice partial sums) and the log
- * probabilities (partial results of a row split over workgroups): not split where the parts do not fit, and in
- * plow_moe_exec_noalloc, which has no such block. Graphs captured from one context share the block too: replay them
+ * many: kept on their plain form when they do not fit), the dense int4 products (K-slice partial sums, in the first
+ * PLOW_MOE_STAGE_DEFAULT_BYTES however large the block is) and the log probabilities (partial results of a row split
+ * over workgroups, a few megabytes at most): not split where the parts do not fit, and in plow_moe_exec_noalloc, which
+ * has no such block. Graphs captured from one context share the block too: replay them
  * one after the other, or capture each from a context of its own. */
 #define PLOW_MOE_STAGE_DEFAULT_BYTES (32u << 20)
 int plow_moe_reserve_staging(PlowMoeCtx* ctx, size_t token_rows, size_t hidden);

@@ -329,7 +329,8 @@ static int run_w4_dense(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, hi
                 aligned(g.out, g.out_f32 ? 4u : 2u),
          "op %u: x and the weights must be 16-byte aligned, scales and output aligned to their elements", (unsigned)in->op);
     if (!launch) return 0;
-    if (c->ws_base && c->stage) g.ws = c->stage, g.ws_bytes = c->stage_bytes;
+    /* what every context holds and no more: a block that has grown would cut K differently, in sums of another order */
+    if (c->ws_base && c->stage) g.ws = c->stage, g.ws_bytes = PLOW_MOE_STAGE_DEFAULT_BYTES;
     return launch_w4(g, glu, st);
 }
 

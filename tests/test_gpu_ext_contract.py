@@ -50,3 +50,25 @@ def test_logits_further_apart_than_a_type_reaches(moe, V, dtype, scale):
         got = got.cpu().double()
         assert torch.isfinite(got).all(), (k, got)
         assert ((got - want[k]).abs() <= 3 * ec.EPS_F32 * want[k].abs()).all(), (k, got, want[k])
+
+
+@pytest.mark.parametrize("M,N,K,glu", [(300, 14336, 8192, False), (1000, 2100, 14336, True), (700, 4096, 14336, False), (90, 7168, 7168, False)])
+def test_same_bits_whatever_staging_the_context_holds(M, N, K, glu):
+    """A larger staging block does not cut a dense call differently."""
+    from plow_amd.lib import Moe
+    print(f"[case] staging M={M} N={N} K={K} glu={glu}", flush=True)
+    moe, g = Moe(0), ec.gen(M)
+    a, b = (tuple(t.cuda() for t in ec.weights(g, (), N, K, 128, True, "bf16")) for _ in range(2))
+    x = torch.randn(M, K, generator=g).to(torch.bfloat16).cuda()
+    outs = []
+    for grow in (0, 1):
+        if grow:
+            moe.reserve_staging(1 << 14, 1 << 15)            # 285 MB
+        o = torch.zeros(M, N, dtype=torch.bfloat16 if glu else torch.float32, device="cuda")
+        inst = (abi.inst(abi.OP_X_GEMM_GLU_W4, t=[0, 1, 2, 3, 4, 5, 6, 7], i=[M, N, K, 128, 0, abi.ACT_SILU]) if glu else
+                abi.inst(abi.OP_X_GEMM_W4, t=[0, 1, 2, 3, 4], i=[M, N, K, 128, 0, 0, 1]))
+        moe.exec(inst, ec.table_of([o, x, *a, *b]))
+        torch.cuda.synchronize()
+        outs.append(o.cpu())
+    assert torch.equal(outs[0], outs[1]), (outs[0].float() - outs[1].float()).abs().max()
+    moe.close()
