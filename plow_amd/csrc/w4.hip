@@ -167,14 +167,26 @@ __global__ __launch_bounds__(V_WAVES* WAVE) void k_w4_vec(GroupW4 g, uint32_t ch
 #define W4_VEC_MAX_K 8192u
 /* Which calls take the matrix-vector form: one dense row, or a few routing slots, each of which streams its expert's
  * weights by itself (and needs no sort). Measured against the tiles of 16 rows: dense 120001 x 4096 45 us for 58, 2048 x
- * 2816 6.4 for 8.8, 7168 x 7168 10.2 for 12.3 (two rows, one after the other: 86 for 60, 6.4 for 8.8, 17.8 for 12.7);
- * 64 slots over 128 experts of 4096 x 1536 126 us for 144, over 384 of 7168 x 2048 289 for 350; 128 slots over the 128
- * experts 227 for 194. */
+ * 2816 6.4 for 8.8, 7168 x 7168 10.2 for 12.3 (two rows, one after the other: 86 for 60, 6.4 for 8.8, 17.8 for 12.7).
+ * Slots: GLU and DOWN of random routing in us, matrix-vector / tiles (rows of experts, top 2 to 8):
+ *                     4096 x 1536, G 128                        7168 x 2048, G 32                       2048 x 1408, G 64
+ *   E       16 slots 24      32       48      64   |  16       24       32       48       64   |  16     24     32     48     64
+ *     1,2    32/93  46/93   56/93   82/99 101/99   | 71/200 117/200  127/203  206/208  238/208 | 20/76  30/76  32/76  51/81  54/80
+ *     4      33/51  47/51   56/52   84/53 102/57   | 70/102 117/102  127/103  207/104  245/109 | 20/41  30/41  32/41  51/42  55/45
+ *     8      35/45  49/46   56/47   85/48 104/48   | 74/85  116/86   131/88   215/89   251/89  | 21/37  30/38  32/38  50/38  55/39
+ *    16      37/53  49/55   58/56   87/58 105/58   | 78/102 116/106  137/117  214/120  256/121 | 22/41  31/42  33/43  50/43  55/44
+ *    32      38/60  47/63   61/65   83/67 112/79   | 79/127 116/139  140/143  215/156  263/195 | 22/48  30/50  34/51  50/53  58/54
+ *    64      37/60  51/62   63/74   86/95 113/109  | 81/131 117/142  144/194  214/222  271/240 | 22/49  30/50  34/52  49/63  59/66
+ *   128      37/60  49/63   61/87   90/107 116/121 | 83/132 117/151  147/200  219/261  278/302 | 21/50  29/51  33/52  47/72  60/75
+ * The more slots share an expert, the sooner the tiles win, which read it once: from 20 slots and one more per two
+ * experts on (never past 64: 128 slots over 128 experts of 4096 x 1536 227 us for 194; of two experts the tiles have too
+ * few workgroups to win below that). Off the best by up to a third around 24 slots of 8 experts, to either side. */
 #define W4_VEC_MAX_SLOTS 64u
 
 bool w4_vec_serves(const GroupW4& g) {
     if (g.K > W4_VEC_MAX_K || g.meta) return false;
-    return g.tab ? g.nslot <= W4_VEC_MAX_SLOTS : g.M == 1u;
+    if (!g.tab) return g.M == 1u;
+    return g.nslot <= W4_VEC_MAX_SLOTS && (g.E <= 2u || g.nslot <= 20u + g.E / 2u);
 }
 
 template <int ITER, bool GLU>

@@ -72,3 +72,35 @@ def test_same_bits_whatever_staging_the_context_holds(M, N, K, glu):
         outs.append(o.cpu())
     assert torch.equal(outs[0], outs[1]), (outs[0].float() - outs[1].float()).abs().max()
     moe.close()
+
+
+def experts(E, H, I, G, seed):
+    g = ec.gen(seed)
+    sets = [tuple(t.cuda() for t in ec.weights(g, (E,), n, k, G, True, "bf16", 0.02)) for n, k in ((I, H), (I, H), (H, I))]
+    return sets, [torch.tensor([[s[c][e].data_ptr() for s in sets] for e in range(E)], dtype=torch.int64).cuda() for c in range(3)]
+
+
+@pytest.mark.parametrize("E,slots,tiles", [(4, 48, True), (8, 64, True), (16, 64, True), (32, 64, True), (8, 16, False), (64, 48, False)])
+def test_slots_that_share_experts_run_as_tiles(moe, E, slots, tiles):
+    """Slot-major experts of a few slots each stream their expert by themselves only while few slots share one: with more
+    of them the rows run as the tiles of a larger batch do, bit for bit."""
+    print(f"[case] shared experts E={E} slots={slots}", flush=True)
+    H, I, G, k = 2048, 512, 64, 2
+    sets, tabs = experts(E, H, I, G, 4)
+    T = slots // k
+    eid = torch.rand(T, E, generator=ec.gen(E)).topk(k, dim=1).indices.to(torch.int32)
+    x = torch.randn(33, H, generator=ec.gen(6)).to(torch.bfloat16).cuda()
+    got = []
+    for rows in (T, 33):                                     # 66 slots always run as tiles; the rows behind T are padding
+        e2 = torch.full((rows, k), -1, dtype=torch.int32)
+        e2[:T] = eid
+        gate = torch.full((rows, k), 0.75)
+        tab = torch.stack([e2, gate.view(torch.int32)], 2).reshape(rows * k, 2).contiguous().cuda()
+        fu, part = torch.zeros(rows * k, I, dtype=torch.bfloat16, device="cuda"), torch.zeros(rows * k, H, device="cuda")
+        moe.exec_many([abi.inst(abi.OP_MOE_GROUP_GLU_FP8_BLK, t=[0, 1, 2, 3, 4, 5], i=[rows * k, I, H, E, k, abi.ACT_SILU, abi.ENC_INT4G, G]),
+                       abi.inst(abi.OP_MOE_GROUP_DOWN_FP8_BLK, t=[6, 0, 2, 3, 4, 5], i=[rows * k, H, I, E, 0, 0, abi.ENC_INT4G, G])],
+                      ec.table_of([fu, x, tab, *tabs, part]))
+        torch.cuda.synchronize()
+        got.append((fu[:slots].cpu(), part[:slots].cpu()))
+    assert (torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])) == tiles
+    assert (got[0][1].double() - got[1][1].double()).norm() <= 2.0 ** -8 * got[1][1].double().norm()
