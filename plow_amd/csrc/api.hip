@@ -271,7 +271,7 @@ static int launch_w8a8(PlowMoeCtx* c, const Hint& h, uint32_t slots, GroupW8A8& 
         return glu ? launch_group_glu_w8a8(g, st) : launch_group_down_w8a8(g, st);
     }
     uint32_t* const word = next_form_word(c);
-    int rc = launch_pick_form(word, g.meta, g.E, st);
+    int rc = launch_pick_form(word, g.meta, g.E, 16u * g.E, st);
     if (rc) return rc;
     g.form_word = word;
     g.form_want = 0u;
@@ -390,6 +390,7 @@ static int run_w4_grouped(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, 
     if (rc) return rc;
     NEED(c, aligned(g.x, 16u), "op %u: t1 must be 16-byte aligned", (unsigned)in->op);
     if (!launch) return 0;
+    if (!g.slots && h.form != 0) g.form_ws = next_form_word(c); /* unknown rows: the form is chosen on the device */
     return launch_w4(g, glu, st);
 }
 

@@ -998,7 +998,7 @@ static bool a16_tiled_try(const GroupA16& g, hipStream_t st, int* rc, bool behin
     if (!group_w8a8_tiled_serves(w)) return false;
     if (behind_choice) {
         if (!GLU && g.a_idx) return false; /* slot-major rows need the slot count, which such a caller states */
-        *rc = launch_pick_form(g.form_ws, g.meta, g.E, st);
+        *rc = launch_pick_form(g.form_ws, g.meta, g.E, 16u * g.E, st);
         if (*rc) return true;
         w.form_word = g.form_ws, w.form_want = 1u;
     }

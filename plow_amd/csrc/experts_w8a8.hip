@@ -732,7 +732,7 @@ int plow_moe_w8a8_setup() {
 
 /* The device-side choice between the streaming and the tiled form of a grouped op whose caller states no row
  * count: one workgroup adds up the experts' row counts. */
-__global__ __launch_bounds__(256) void k_pick_form(uint32_t* word, const int32_t* meta, uint32_t E) {
+__global__ __launch_bounds__(256) void k_pick_form(uint32_t* word, const int32_t* meta, uint32_t E, uint32_t from) {
     __shared__ uint32_t part[4];
     uint32_t s = 0;
     for (uint32_t e = threadIdx.x; e < E; e += 256u) s += (uint32_t)meta[E + e];
@@ -740,11 +740,11 @@ __global__ __launch_bounds__(256) void k_pick_form(uint32_t* word, const int32_t
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63u) == 0u) part[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0u) *word = (part[0] + part[1] + part[2] + part[3] >= 16u * E) ? 1u : 0u;
+    if (threadIdx.x == 0u) *word = (part[0] + part[1] + part[2] + part[3] >= from) ? 1u : 0u;
 }
-int launch_pick_form(uint32_t* word, const int32_t* meta, uint32_t E, hipStream_t st) {
+int launch_pick_form(uint32_t* word, const int32_t* meta, uint32_t E, uint32_t from, hipStream_t st) {
     if (!word || !meta || !E) return PLOW_MOE_EINVAL;
-    k_pick_form<<<1, 256, 0, st>>>(word, meta, E);
+    k_pick_form<<<1, 256, 0, st>>>(word, meta, E, from);
     return 0;
 }
 

@@ -121,9 +121,9 @@ __device__ __forceinline__ bool form_is_mine(const G& g) {
     return form == g.form_want;
 }
 #endif
-/* *word = 1 when meta counts at least 16 routed rows per expert on average (the tiled forms' side of the
- * measured crossover), else 0 */
-int launch_pick_form(uint32_t* word, const int32_t* meta, uint32_t E, hipStream_t st);
+/* *word = 1 when meta counts at least `from` routed rows (the tiled forms' side of the measured crossover: 16 per
+ * expert on average for the fp8 and bf16 kernels), else 0 */
+int launch_pick_form(uint32_t* word, const int32_t* meta, uint32_t E, uint32_t from, hipStream_t st);
 int launch_group_glu_w8a8(const GroupW8A8& g, hipStream_t st);
 int launch_group_down_w8a8(const GroupW8A8& g, hipStream_t st);
 /* the many-rows-per-expert form of the same two ops (block mode only) */
@@ -236,6 +236,11 @@ struct GroupW4 {
     /* scratch for partial sums of a K split (NULL: never split) */
     void* ws;
     size_t ws_bytes;
+    /* rows by meta whose count the host does not know: a word for the choice of the form on the device, and, on the
+     * launches behind it, that word and the form's own value (see GroupW8A8::form_word) */
+    uint32_t* form_ws;
+    const uint32_t* form_word;
+    uint32_t form_want;
 };
 /* the matrix-vector form serves this call (routed experts: straight from the table, no sort) */
 bool w4_vec_serves(const GroupW4& g);

@@ -317,6 +317,7 @@ __global__ __launch_bounds__(C::THREADS, C::MTW == 1 ? 3 : 1) void k_w4_rows(Gro
         w4_rows_tile<C>(g, tl, w4_lds, 0u, 0u, g.M, blockIdx.y * C::TM, n0, blockIdx.z);
         return;
     }
+    if (!form_is_mine(g)) return;
     const uint32_t e = blockIdx.y, cnt = (uint32_t)g.meta[g.E + e], r0 = (uint32_t)g.meta[e];
     if (cnt == 0u) return;
     for (int st = 0; st < (C::GLU ? 2 : 1); st++) {

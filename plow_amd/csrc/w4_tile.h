@@ -421,6 +421,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_w4_tile(GroupW4 g, W4Tiles tl
     extern __shared__ __attribute__((aligned(16))) uint8_t w4_lds[];
     constexpr bool EXPERTS = C::TM == (int)PLOW_MPF_BM; /* meta counts tiles of that many rows */
     const bool routed = EXPERTS && g.meta;
+    if (routed && !form_is_mine(g)) return;
     const int32_t* const tilep = g.meta + 2u * g.E;
     const uint32_t n0 = blockIdx.x * C::TN, lane = threadIdx.x & 63u, total = routed ? (uint32_t)tilep[g.E] : gridDim.y;
     uint32_t e = 0u, r0 = 0u, cnt = g.M;

@@ -104,3 +104,51 @@ def test_slots_that_share_experts_run_as_tiles(moe, E, slots, tiles):
         got.append((fu[:slots].cpu(), part[:slots].cpu()))
     assert (torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])) == tiles
     assert (got[0][1].double() - got[1][1].double()).norm() <= 2.0 ** -8 * got[1][1].double().norm()
+
+
+@pytest.mark.parametrize("form", ["one by one", "one by one, captured", "segment"])
+@pytest.mark.parametrize("T,E,k", [(333, 4, 2), (700, 3, 1), (30, 8, 2), (3, 8, 2), (97, 8, 2), (96, 8, 2)])
+def test_gathered_experts_without_a_stated_count(moe, T, E, k, form):
+    """Ops 85 / 86 whose caller states no row count: the form is chosen on the device from the routing meta and the bytes
+    are those of the run that states the count (24 rows of an expert on average lie on one side, more on the other)."""
+    print(f"[case] unstated T={T} E={E} k={k} {form}", flush=True)
+    H, I, G = 2176, 1152, 64
+    sets, tabs = experts(E, H, I, G, 3)
+    eid = torch.rand(T, E, generator=ec.gen(T)).topk(k, dim=1).indices.to(torch.int32)
+    gate = torch.rand(T, k, generator=ec.gen(2)) + 0.1
+    tab = torch.stack([eid, gate.view(torch.int32)], 2).reshape(T * k, 2).contiguous().cuda()
+    x = torch.randn(T, H, generator=ec.gen(5)).to(torch.bfloat16).cuda()
+    R = abi.max_rows(T, k, E)
+    maps = [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (3 * E + 1, R, R, R)]
+    fu, part = torch.zeros(R, I, dtype=torch.bfloat16, device="cuda"), torch.zeros(T * k + 1, H, device="cuda")
+    tensors = ec.table_of([fu, x, tab, *tabs, part, *maps])
+
+    def ops(n):
+        return [abi.inst(abi.OP_MOE_GROUP_GLU_PF, t=[0, 1, 3, 4, 7, 8, 5], i=[I, H, E, abi.ENC_INT4G, 0, abi.ACT_SILU, G, abi.ARM_A16], slots=n),
+                abi.inst(abi.OP_MOE_GROUP_DOWN_PF, t=[6, 0, 3, 4, 7, 5, 9, 10], i=[H, I, E, abi.ENC_INT4G, 0, 0, G, abi.ARM_A16], slots=n)]
+    moe.exec(abi.inst(abi.OP_MOE_ALIGN_PF, t=[7, 2, 8, 9, 10], i=[T, E, k]), tensors)
+    got = []
+    for n in (T * k, 0):
+        fu.fill_(3.0), part.fill_(3.0)
+        run = ops(n)
+        torch.cuda.synchronize()
+        if n or form == "one by one":
+            for d in run:
+                moe.exec(d, tensors)
+        elif form == "segment":
+            moe.pf(run, tensors, T)
+        else:
+            side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+            with torch.cuda.stream(side):
+                graph.capture_begin()
+                for d in run:
+                    moe.exec(d, tensors, side.cuda_stream)
+                graph.capture_end()
+            for _ in range(3):
+                fu.fill_(3.0), part.fill_(3.0)
+                graph.replay()
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        got.append((fu.cpu(), part.cpu()))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    assert (got[1][1][-1] == 3).all()
