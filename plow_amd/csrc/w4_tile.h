@@ -345,10 +345,14 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
                             t[i][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mt], b, from, 0, 0, 0);
                         }
                     }
-                    /* the four-wave forms do not fit their registers with more reads moved up: 64 rows of 7168 x 7168 31 us for
-                     * 27.5, a GLU of groups of 64 with zero points 850 for 819; but for the GLU of groups of 128 without: 176
-                     * for 183. (The eight-wave forms do; groups of 32 take 239 us for 218 with it.) */
-                    if (C::WT == 1 && !(NS == 2 && G == 128 && !C::ASYM)) __builtin_amdgcn_sched_barrier(0);
+                    /* Whether reads may move up over an instruction's products, in the four-wave forms (the eight-wave forms
+                     * let them; their groups of 32 take 239 us for 218 without). us let / held back, for 64 rows of 7168 x
+                     * 7168, a GLU of 64 rows of 4096 x 7168, and 512 and 2048 tokens over 64 experts of 2048 x 1408, top 6:
+                     *   G 32     37.9 38.3   31.4 32.7   285 305   818 878     zero points  37.3 37.3   41.5 42.1   366 373   1085 1126
+                     *   G 64     32.3 32.4   28.3 28.3   256 259   716 728     zero points  33.9 32.9   32.1 31.1   304 298    845  825
+                     *   G 128    31.2 27.8   28.7 27.4   189 184   482 454     zero points  30.8 29.1   29.0 28.4   270 261    756  733
+                     * G 128 without zero points is best with the GLU's let and the plain product's held back (175 and 458). */
+                    if (C::WT == 1 && (C::ASYM ? G != 32 : G == 128 && NS == 1)) __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
                 for (int i = 0; i < TILES; i++) {
