@@ -163,7 +163,9 @@ __global__ __launch_bounds__(V_WAVES* WAVE) void k_w4_vec(GroupW4 g, uint32_t ch
     }
 }
 
-/* a lane holds its share of the row: 64 registers at 8192 columns */
+/* a lane holds its share of the row: 64 registers at 8192 columns. Longer rows run as a tile of 16 with K split: 4096 x
+ * 8192, G = 128, takes 7.3 us here, 4096 x 11008 13.4 us and 4096 x 14336 15.1 us there (2 TB/s; two launches), 7168 x
+ * 18432, G = 32, 22.8 us, 8192 x 28672 30.8 us (3.9 TB/s) */
 #define W4_VEC_MAX_K 8192u
 /* Which calls take the matrix-vector form: one dense row, or a few routing slots, each of which streams its expert's
  * weights by itself (and needs no sort). Measured against the tiles of 16 rows: dense 120001 x 4096 45 us for 58, 2048 x

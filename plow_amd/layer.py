@@ -349,6 +349,12 @@ class HeadConfig:
 
 def plan_head(cfg: HeadConfig) -> LayerPlan:
     """Emit the chain RMSNorm (1) -> logits (180, or the int4 product) -> log probabilities (0x7010)."""
+    if cfg.enc not in ("bf16", "int4g"):
+        raise ValueError(f"a head's weights are bf16 or int4g, not {cfg.enc}")
+    if not 1e-30 <= cfg.scale <= 1e30:         # (the op reads 0 as 1)
+        raise ValueError(f"the factor on the logits must lie in 1e-30 .. 1e30, not {cfg.scale}")
+    if cfg.n_alt > abi.LOGPROB_MAX_ALT:
+        raise ValueError(f"at most {abi.LOGPROB_MAX_ALT} most likely tokens per row, not {cfg.n_alt}")
     p = LayerPlan(cfg)
     T, H, V = cfg.T, cfg.H, cfg.V
     x = p._t("x", "bf16", (T, H), "in")
