@@ -233,14 +233,10 @@ struct GroupW4 {
      * no expert serves are zeroed (DOWN) */
     const void* tab;
     uint32_t nslot, kx, zero_unserved;
-    /* scratch for partial sums of a K split (NULL: never split) */
+    /* scratch: dense calls, for partial sums of a K split (NULL: never split); rows by meta whose count the host does not
+     * know, the word for the choice of the form on the device (see GroupW8A8::form_word; NULL: tiles of 16 rows) */
     void* ws;
     size_t ws_bytes;
-    /* rows by meta whose count the host does not know: a word for the choice of the form on the device, and, on the
-     * launches behind it, that word and the form's own value (see GroupW8A8::form_word) */
-    uint32_t* form_ws;
-    const uint32_t* form_word;
-    uint32_t form_want;
 };
 /* the matrix-vector form serves this call (routed experts: straight from the table, no sort) */
 bool w4_vec_serves(const GroupW4& g);

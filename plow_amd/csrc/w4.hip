@@ -326,23 +326,20 @@ int launch_w4(const GroupW4& g, bool glu, hipStream_t st) {
         k_w4_tiny<<<dim3((g.N + 63u) / 64u, g.E, z), 64, 0, st>>>(g, glu ? 1u : 0u);
         return 0;
     }
-    if (g.form_ws && !g.slots && plow_moe_tuning().form_on_device) {
+    if (g.meta && g.ws) {
         /* the rows are known to the device only: both sides of the rule below go out behind its count (tiles of 16 rows
          * up to 24 rows per expert on average, else of 64), and the one that it does not name returns at once. Ops one at
          * a time over 64 experts of 2048 x 1408, top 6, always tiles of 16 / so / with the count stated: 2048 tokens GLU
          * 496 / 266 / 281 us, DOWN 360 / 164 / 160; 512 tokens 158 / 102 / 103 and 105 / 76 / 73; one token, where the
          * count and the launch that returns are for nothing, 16 / 21 / 17 and 9 / 14 / 9. */
-        int rc = launch_pick_form(g.form_ws, g.meta, g.E, 24u * g.E + 1u, st);
+        int rc = launch_pick_form((uint32_t*)g.ws, g.meta, g.E, 24u * g.E + 1u, st);
         if (rc) return rc;
-        GroupW4 o = g;
-        o.form_ws = nullptr, o.form_word = g.form_ws, o.form_want = 0u;
-        W4Plan p = w4_shape(o, glu, 16u, 0u, n_cu);
-        rc = w4_rows_launch(o, W4Tiles{}, glu, p.wide, p.tm, dim3(p.nt, o.E), st);
+        W4Plan p = w4_shape(g, glu, 16u, 0u, n_cu);
+        rc = w4_rows_launch(g, W4Tiles{}, glu, p.wide, p.tm, dim3(p.nt, g.E), st);
         if (rc) return rc;
-        o.form_want = 1u;
-        p = w4_shape(o, glu, 64u, 0u, n_cu);
+        p = w4_shape(g, glu, 64u, 0u, n_cu);
         const uint32_t gy = (8u * n_cu + p.nt - 1u) / p.nt; /* (whatever it is, the workgroups walk all row tiles) */
-        return w4_tiled_launch(o, W4Tiles{}, glu, p.tm, dim3(p.nt, gy), st);
+        return w4_tiled_launch(g, W4Tiles{}, glu, p.tm, dim3(p.nt, gy), st);
     }
     W4Tiles tl = {};
     W4Plan p;

@@ -308,8 +308,10 @@ __device__ __forceinline__ void w4_rows_tile(const GroupW4& g, const W4Tiles& tl
         }
 }
 
-/* grid: x = channel tiles, y = dense row tile or expert (its row tiles one after the other), z = K slice */
-template <class C>
+/* grid: x = channel tiles, y = dense row tile or expert (its row tiles one after the other), z = K slice. CHOICE: behind
+ * a choice made on the device (instances of their own: with the test in all of them the GLU of groups of 128 with zero
+ * points needs four registers more than it has, and 64 tokens over 128 experts take 316 us for 298) */
+template <class C, bool CHOICE>
 __global__ __launch_bounds__(C::THREADS, C::MTW == 1 ? 3 : 1) void k_w4_rows(GroupW4 g, W4Tiles tl) {
     extern __shared__ __attribute__((aligned(16))) uint8_t w4_lds[];
     const uint32_t n0 = blockIdx.x * C::TN;
@@ -317,7 +319,7 @@ __global__ __launch_bounds__(C::THREADS, C::MTW == 1 ? 3 : 1) void k_w4_rows(Gro
         w4_rows_tile<C>(g, tl, w4_lds, 0u, 0u, g.M, blockIdx.y * C::TM, n0, blockIdx.z);
         return;
     }
-    if (!form_is_mine(g)) return;
+    if (CHOICE && !w4_chosen(g, 0u)) return;
     const uint32_t e = blockIdx.y, cnt = (uint32_t)g.meta[g.E + e], r0 = (uint32_t)g.meta[e];
     if (cnt == 0u) return;
     for (int st = 0; st < (C::GLU ? 2 : 1); st++) {
@@ -348,12 +350,22 @@ static int by_form(const GroupW4& g, bool glu, bool wide, uint32_t rows, F&& f) 
 /* workgroups of the kernel that a CU holds, asked once */
 template <class C>
 static int rows_per_cu = 1;
+/* the forms that a choice on the device is made for: tiles of 16 rows x 64 channels */
+template <class C>
+static constexpr bool behind_choice = C::MTW == 1 && (C::GLU || C::NS == 1);
 
 int w4_rows_launch(const GroupW4& g, const W4Tiles& tl, bool glu, bool wide, uint32_t rows, dim3 grid, hipStream_t st) {
     return by_form(g, glu, wide, rows, [&](auto c) {
         using C = decltype(c);
-        k_w4_rows<C><<<grid, C::THREADS, C::LDS, st>>>(g, tl);
-        return 0;
+        if (!g.meta || !g.ws) {
+            k_w4_rows<C, false><<<grid, C::THREADS, C::LDS, st>>>(g, tl);
+            return 0;
+        }
+        if constexpr (behind_choice<C>) {
+            k_w4_rows<C, true><<<grid, C::THREADS, C::LDS, st>>>(g, tl);
+            return 0;
+        }
+        return (int)PLOW_MOE_EINVAL;
     });
 }
 int w4_rows_per_cu(const GroupW4& g, bool glu, bool wide, uint32_t rows) {
@@ -362,7 +374,10 @@ int w4_rows_per_cu(const GroupW4& g, bool glu, bool wide, uint32_t rows) {
 
 template <class C>
 static bool setup1() {
-    const void* const k = (const void*)k_w4_rows<C>;
+    const void* const k = (const void*)k_w4_rows<C, false>;
+    if constexpr (behind_choice<C>) {
+        if (hipFuncSetAttribute((const void*)k_w4_rows<C, true>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS) != hipSuccess) return false;
+    }
     return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS) == hipSuccess &&
            hipOccupancyMaxActiveBlocksPerMultiprocessor(&rows_per_cu<C>, k, C::THREADS, C::LDS) == hipSuccess && rows_per_cu<C> > 0;
 }

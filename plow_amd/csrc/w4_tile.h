@@ -35,6 +35,11 @@ struct W4Tiles {
     float* part;
 };
 
+/* whether the choice behind which a launch of routed experts went out names its form: 0 tiles of 16 rows, 1 of 64 */
+__device__ __forceinline__ bool w4_chosen(const GroupW4& g, uint32_t form) {
+    return *(const __attribute__((address_space(4))) uint32_t*)g.ws == form; /* written by an earlier kernel: a scalar load */
+}
+
 __device__ __forceinline__ float w4_f32(uint32_t h, uint32_t f16) {
     asm("" : "+v"(f16)); /* a select, no branch */
     return f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : __uint_as_float(h << 16);
@@ -419,13 +424,13 @@ __device__ __forceinline__ void w4_tile(const GroupW4& g, const W4Tiles& tl, uin
 }
 
 /* grid: x = channel tiles, y = row tiles (routed experts: over all of them, from gridDim.y on the workgroups take
- * another), z = K slice */
-template <class C>
+ * another), z = K slice. CHOICE: routed experts behind a choice made on the device */
+template <class C, bool CHOICE>
 __global__ __launch_bounds__(C::THREADS, 2) void k_w4_tile(GroupW4 g, W4Tiles tl) {
     extern __shared__ __attribute__((aligned(16))) uint8_t w4_lds[];
     constexpr bool EXPERTS = C::TM == (int)PLOW_MPF_BM; /* meta counts tiles of that many rows */
     const bool routed = EXPERTS && g.meta;
-    if (routed && !form_is_mine(g)) return;
+    if (CHOICE && !w4_chosen(g, 1u)) return;
     const int32_t* const tilep = g.meta + 2u * g.E;
     const uint32_t n0 = blockIdx.x * C::TN, lane = threadIdx.x & 63u, total = routed ? (uint32_t)tilep[g.E] : gridDim.y;
     uint32_t e = 0u, r0 = 0u, cnt = g.M;
@@ -458,7 +463,10 @@ static int w4_per_cu = 1;
 
 template <class C>
 static bool w4_setup() {
-    const void* const k = (const void*)k_w4_tile<C>;
+    const void* const k = (const void*)k_w4_tile<C, false>;
+    if constexpr (C::TM == (int)PLOW_MPF_BM) {
+        if (hipFuncSetAttribute((const void*)k_w4_tile<C, true>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS) != hipSuccess) return false;
+    }
     return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS) == hipSuccess &&
            hipOccupancyMaxActiveBlocksPerMultiprocessor(&w4_per_cu<C>, k, C::THREADS, C::LDS) == hipSuccess && w4_per_cu<C> > 0;
 }

@@ -35,8 +35,15 @@ static int by_form(const GroupW4& g, bool glu, uint32_t rows, F&& f) {
 int w4_tiled_launch(const GroupW4& g, const W4Tiles& tl, bool glu, uint32_t rows, dim3 grid, hipStream_t st) {
     return by_form(g, glu, rows, [&](auto c) {
         using C = decltype(c);
-        k_w4_tile<C><<<grid, C::THREADS, C::LDS, st>>>(g, tl);
-        return 0;
+        if (!g.meta || !g.ws) {
+            k_w4_tile<C, false><<<grid, C::THREADS, C::LDS, st>>>(g, tl);
+            return 0;
+        }
+        if constexpr (C::TM == (int)PLOW_MPF_BM) {
+            k_w4_tile<C, true><<<grid, C::THREADS, C::LDS, st>>>(g, tl);
+            return 0;
+        }
+        return (int)PLOW_MOE_EINVAL;
     });
 }
 int w4_tiled_per_cu(const GroupW4& g, bool glu, uint32_t rows) {
