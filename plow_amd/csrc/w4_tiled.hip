@@ -2,14 +2,16 @@
  * channels of gate and up), a wave per 64 rows x 64 weight rows, so that a weight unpacked feeds four matrix
  * instructions and a row read from LDS four.
  *
- * 2048 x 4096 x 7168, G = 128: 135 us = 889 TFLOP/s (a library product of bf16 by bf16 reaches 1314 at 8192 cubed);
- * the same with groups of 32 and zero points 218 us. 512 tokens over 64 experts of 2048 x 1408, top 6: 102 us for gate and
- * up, 55 for down (230 and 320 TFLOP/s: 48 of a tile's 64 rows count, and the tiles come to 1.4 and just over 1 rounds of
- * what the chip holds). Bound by a SIMD's two waves waiting on LDS and on their barrier: the matrix units are busy 39 %
- * of the time, the vector units (unpacking, scaling, x staged anew by every channel tile) 58 %, LDS 41 %; without
- * staging and loads 133 of 156 us are left. Tried and slower (2048 x 4096 x 7168 at 145 us): staging the next step between
- * this one's products 183 us, waves of 128 x 64 at one per SIMD 195, two steps on their way 382, none of which fits the
- * registers; row tiles of one XCD side by side 155 for 156. */
+ * 2048 x 4096 x 7168, G = 128: 133 us = 903 TFLOP/s (a library product of bf16 by bf16 reaches 1314 at 8192 cubed), the
+ * GLU of 2048 x 2048 x 7168 135 us; the products with groups of 32 and zero points 218 us both. 512 tokens over 64 experts
+ * of 2048 x 1408, top 6: 102 us for gate and up, 55 for down (347 and 322 TFLOP/s: 48 of a tile's 64 rows count, and the
+ * tiles come to 1.4 and just over 1 rounds of what the chip holds). Bound by a SIMD's two waves waiting on LDS and on their
+ * barrier: the matrix units are busy 39 % of the time, the vector units (unpacking, scaling, x staged anew by every channel
+ * tile) 58 %, LDS 41 % (under the profiler, where the first call takes 156 us). Groups of 32 have a matrix instruction
+ * beside four scaling ones and, with zero points, four more that multiply its C operand. Tried and slower, each beside
+ * what the first call took at the time: staging the next step between this one's products 183 us for 145, waves of 128 x
+ * 64 at one per SIMD 195 for 145, two steps on their way 382 for 145, none of which fits the registers; row tiles of one
+ * XCD side by side 155 for 156. */
 #include "w4_forms.h"
 #include "w4_tile.h"
 
