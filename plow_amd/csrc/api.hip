@@ -390,7 +390,8 @@ static int run_w4_grouped(PlowMoeCtx* c, const PlowDevInst* in, void* const* T, 
     if (rc) return rc;
     NEED(c, aligned(g.x, 16u), "op %u: t1 must be 16-byte aligned", (unsigned)in->op);
     if (!launch) return 0;
-    if (!g.slots && h.form != 0 && plow_moe_tuning().form_on_device) g.ws = next_form_word(c), g.ws_bytes = sizeof(uint32_t); /* unknown rows: the form is chosen on the device */
+    /* unknown rows: the form is chosen on the device (not without a context, whose word all calls on a GPU would share) */
+    if (!g.slots && h.form != 0 && c->ws_base && plow_moe_tuning().form_on_device) g.ws = next_form_word(c), g.ws_bytes = sizeof(uint32_t);
     return launch_w4(g, glu, st);
 }
 

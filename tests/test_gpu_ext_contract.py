@@ -152,3 +152,37 @@ def test_gathered_experts_without_a_stated_count(moe, T, E, k, form):
         got.append((fu.cpu(), part.cpu()))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
     assert (got[1][1][-1] == 3).all()
+
+
+def test_gathered_experts_without_a_context_choose_nothing_on_the_device(moe):
+    """plow_moe_exec_noalloc has one workspace for all calls on a GPU: ops 85 / 86 use nothing of it, so that calls on
+    several streams may overlap, each with the bytes of the form for few rows."""
+    E, k, H, I, G = 4, 2, 2176, 1152, 64
+    sets, tabs = experts(E, H, I, G, 9)
+    jobs = []
+    for T in (6, 300, 500, 9):
+        eid = torch.rand(T, E, generator=ec.gen(T)).topk(k, dim=1).indices.to(torch.int32)
+        tab = torch.stack([eid, torch.full((T, k), 0.5).view(torch.int32)], 2).reshape(T * k, 2).contiguous().cuda()
+        x = torch.randn(T, H, generator=ec.gen(5)).to(torch.bfloat16).cuda()
+        R = abi.max_rows(T, k, E)
+        maps = [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (3 * E + 1, R, R, R)]
+        fu, part = torch.zeros(R, I, dtype=torch.bfloat16, device="cuda"), torch.zeros(T * k, H, device="cuda")
+        keep = [fu, x, tab, *tabs, part, *maps]
+        tensors = ec.table_of(keep)
+        pair = [abi.inst(abi.OP_MOE_GROUP_GLU_PF, t=[0, 1, 3, 4, 7, 8, 5], i=[I, H, E, abi.ENC_INT4G, 0, abi.ACT_SILU, G, abi.ARM_A16]),
+                abi.inst(abi.OP_MOE_GROUP_DOWN_PF, t=[6, 0, 3, 4, 7, 5, 9, 10], i=[H, I, E, abi.ENC_INT4G, 0, 0, G, abi.ARM_A16])]
+        moe.exec(abi.inst(abi.OP_MOE_ALIGN_PF, t=[7, 2, 8, 9, 10], i=[T, E, k]), tensors)
+        assert moe.dec(pair, tensors, T) == 0                # the decode segment: the form for few rows, whatever the count
+        torch.cuda.synchronize()
+        want = (fu.clone(), part.clone())
+        fu.zero_(), part.zero_()
+        jobs.append((pair, tensors, keep, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    err = C.create_string_buffer(256)
+    for _ in range(5):
+        for pair, tensors, _, _, st in jobs:
+            for d in pair:
+                assert moe.lib.plow_moe_exec_noalloc(C.byref(d), tensors, st.cuda_stream, err, 256) == 0, err.value
+    torch.cuda.synchronize()
+    for _, _, keep, want, _ in jobs:
+        assert torch.equal(keep[0], want[0]) and torch.equal(keep[6], want[1])
