@@ -11,8 +11,9 @@
  * experts (4096 x 1536, G = 128, zero points) took 325 us for 288, four steps ahead 555.
  *
  * What it reaches: those experts' gate and up 163 us for 843 MB (5.2 TB/s), their down, whose rows are short (6 steps),
- * 117 us for 421 MB (3.6 TB/s, the launch that zeroes the rows of padding included); 16 rows of 120001 x 4096, G = 64, 67 us for 261 MB (3.9 TB/s); 16 rows of 7168 x 2048,
- * G = 32, where four slices of K and their join are all latency, 8.5 + 3 us. */
+ * 117 us for 421 MB (3.6 TB/s, the launch that zeroes the rows of padding included); 16 rows of 120001 x 4096, G = 64, 67
+ * us for 261 MB (3.9 TB/s); 16 rows of 7168 x 2048, G = 32, where four slices of K and their join are all latency, 8.5 + 3
+ * us. */
 #include "w4_forms.h"
 #include "w4_tile.h"
 
